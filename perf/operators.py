@@ -2,7 +2,7 @@
 
 The cache holds K and V as OCP e4m3 codes in pages of 16 tokens. The 16
 tokens of one KV head are a block; its K codes share one power of two 2^e and
-its V codes another, so a stored value is code * 2^e, with -15 <= e <= 7.
+its V codes another (bf16), so a stored value is code * 2^e, -15 <= e <= 7.
 
   append  a step's new rows of K and V go into their pages. Per block,
           e = the smallest exponent with max|x| <= 448 * 2^e over the block's
@@ -135,9 +135,9 @@ def _sessions(case):
 
 
 def work(case):
-    """append: the new rows in, their codes out, an exponent for each block
-    (read where the block was begun before); with rope q in and out and the
-    tables' rows. attend: q in, out, every cached code and exponent that a
+    """append: the new rows in, their codes out, two bytes of scale for each
+    block's part (read where the block was begun before); with rope q in and out and the
+    tables' rows. attend: q in, out, every cached code and scale that a
     session's queries see, once, and the page ids; flops of the two products."""
     qh, kvh, hd = SHAPES[case["shape"]]
     nbytes = flops = 0
@@ -145,12 +145,12 @@ def work(case):
         pages = -(-(ctx + n) // 16)
         if case["op"] == "append":
             touched = pages - ctx // 16
-            nbytes += n * 2 * kvh * hd * (2 + 1) + (touched + (ctx % 16 > 0)) * kvh * 2 + touched * 4
+            nbytes += n * 2 * kvh * hd * (2 + 1) + (touched + (ctx % 16 > 0)) * kvh * 4 + touched * 4
             if case["rope"]:
                 nbytes += n * (2 * 2 * qh * hd + hd * 4)
                 flops += 3 * n * (qh + kvh) * hd
         else:
-            nbytes += 2 * 2 * n * qh * hd + (ctx + n) * 2 * kvh * hd + pages * (2 * kvh + 4)
+            nbytes += 2 * 2 * n * qh * hd + (ctx + n) * 2 * kvh * hd + pages * (4 * kvh + 4)
             flops += 4 * qh * hd * (n * ctx + n * (n + 1) // 2)
     return {"bytes": nbytes, "flops": flops}
 
@@ -183,6 +183,10 @@ def _exponent(most):
     return torch.where(most > 0, e, torch.full_like(e, -15)).clamp(-15, 7)
 
 
+def _power(e):
+    return torch.ldexp(torch.ones((), device="cuda"), e)
+
+
 def _codes(x, e):
     y = torch.ldexp(x, -e).clamp(-448.0, 448.0)
     return torch.where(y == y, y, torch.zeros_like(y)).to(torch.float8_e4m3fn)
@@ -203,7 +207,7 @@ def _inputs(case, seed):
                         for (ctx, n, _), c in zip(sessions, counts)]).clamp(0, 16)
     order = _order(width)
     blocks = torch.zeros((pages, kvh, 2 * 16 * width), dtype=torch.uint8, device="cuda")
-    exps = torch.zeros((pages, kvh, 2), dtype=torch.int8, device="cuda")
+    scales = torch.zeros((pages, kvh, 2), dtype=torch.bfloat16, device="cuda")
     loud = torch.ones((kvh, 1, hd), device="cuda")
     loud.view(-1)[torch.randperm(kvh * hd, generator=g, device="cuda")[: math.ceil(0.01 * kvh * hd)]] = OUTLIER_GAIN
     live = (torch.arange(16, device="cuda") < cached[:, None])[:, None, :, None]
@@ -217,7 +221,7 @@ def _inputs(case, seed):
         flat = torch.empty((len(ids), kvh, 16 * width), dtype=torch.uint8, device="cuda")
         flat[..., order[part].reshape(-1) - part * 16 * width] = c.reshape(len(ids), kvh, 16 * width)
         blocks[ids, :, part * 16 * width: (part + 1) * 16 * width] = flat
-        exps[ids, :, part] = e.to(torch.int8)
+        scales[ids, :, part] = _power(e).bfloat16()
         del x, c, flat
     rows = sum(n for _, n, _ in sessions)
     kind = torch.bfloat16 if case["rows"] == "bf16" else torch.float16
@@ -227,7 +231,7 @@ def _inputs(case, seed):
     q, k, v = x.split([qh * hd, kvh * hd, kvh * hd], 1)
     if not case["fused"]:
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    got = {"ids": ids, "blocks": blocks, "exps": exps, "order": order, "q": q, "k": k, "v": v, "pages": pages,
+    got = {"ids": ids, "blocks": blocks, "scales": scales, "order": order, "q": q, "k": k, "v": v, "pages": pages,
            "tables": torch.split(ids, counts), "keep": x}
     if case["rope"]:
         for name, n in (("q_bias", qh * hd), ("k_bias", kvh * hd), ("v_bias", kvh * hd)):
@@ -261,9 +265,10 @@ def prepare(case, seed):
         pool = tk.KvPool(1, x["pages"], kvh, hd, tk.KV_E4M3)
         view = pool.layer(0)
         state["blocks"] = torch.as_tensor(_Memory(view.k, tuple(x["blocks"].shape), "|u1", pool), device="cuda")
-        state["exps"] = torch.as_tensor(_Memory(view.k_scales, tuple(x["exps"].shape), "|i1", pool), device="cuda")
+        state["scales"] = torch.as_tensor(_Memory(view.k_scales, tuple(x["scales"].shape), "<i2", pool),
+                                          device="cuda").view(torch.bfloat16)
         state["blocks"].copy_(x["blocks"])
-        state["exps"].copy_(x["exps"])
+        state["scales"].copy_(x["scales"])
         batch = tk.Batch().plan(pool, [tk.Session(ctx, n, t.tolist()) for (ctx, n, _), t in zip(sessions, x["tables"])], qh)
         kind = tk.ROWS_BF16 if case["rows"] == "bf16" else tk.ROWS_F16
         q, k, v, out = x["q"], x["k"], x["v"], state["out"]
@@ -323,14 +328,14 @@ def _append(state):
         x[state["tile"], state["pos"] % 16, :, :hd] = rows.view(-1, kvh, hd)
         x = x.transpose(1, 2)
         e = _exponent(torch.where(x == x, x.abs(), torch.zeros_like(x)).amax((-1, -2)))
-        had = state["exps"][touched, :, part].int()
+        had = torch.frexp(state["scales"][touched, :, part].float())[1] - 1
         e = torch.where(begun[:, None] > 0, torch.maximum(e, had), e)
         at = state["order"][part].reshape(-1)
         was = mine[..., at].view(torch.float8_e4m3fn).float().view(len(touched), kvh, 16, width)
         was = _codes(torch.ldexp(was, had[..., None, None]), e[..., None, None]).view(torch.uint8)
         now = _codes(x, e[..., None, None]).view(torch.uint8)
         mine[..., at] = torch.where(old[:, None, :, None], was, now).reshape(len(touched), kvh, 16 * width)
-        state["exps"][touched, :, part] = e.to(torch.int8)
+        state["scales"][touched, :, part] = _power(e).bfloat16()
     state["blocks"][touched] = mine
     return got
 
@@ -339,7 +344,7 @@ def _values(state, table, part, hd):
     """The rows [KV head][token][dim] that a session's pages hold."""
     width = _block_width(hd)
     c = state["blocks"][table][..., state["order"][part].reshape(-1)].view(torch.float8_e4m3fn).float()
-    c = torch.ldexp(c, state["exps"][table, :, part].int()[..., None])
+    c = c * state["scales"][table, :, part].float()[..., None]
     kvh = c.shape[1]
     return c.view(-1, kvh, 16, width)[..., :hd].transpose(0, 1).reshape(kvh, -1, hd)
 
@@ -374,8 +379,8 @@ def run(state):
         got = _append(state)
     else:
         return _attend(state)
-    # the cache after the step: the codes as the numbers they are, and the exponents
-    return dict(got, codes=state["blocks"].view(torch.float8_e4m3fn), exponents=state["exps"])
+    # the cache after the step: the codes as the numbers they are, and the blocks' powers of two
+    return dict(got, codes=state["blocks"].view(torch.float8_e4m3fn), scales=state["scales"])
 
 
 # ---------------------------------------------------------------------------
@@ -409,7 +414,7 @@ def exact(case, seed):
     if case["op"] == "attend":
         out = torch.empty((x["q"].shape[0], qh * hd), dtype=torch.float64, device="cuda")
         for (ctx, n, row), table in zip(_sessions(case), x["tables"]):
-            bits, power = x["blocks"][table], 2.0 ** x["exps"][table].double()
+            bits, power = x["blocks"][table], x["scales"][table].double()
             pos = ctx + torch.arange(n, device="cuda")
             for head in range(kvh):
                 kv = []
@@ -436,7 +441,7 @@ def exact(case, seed):
 
         q, k, v = rotate(q, x["q_bias"]), rotate(k, x["k_bias"]), v + x["v_bias"].double()
         got["q"] = q
-    codes = _number(x["blocks"])
+    codes, scales = _number(x["blocks"]), x["scales"].double()
     for (ctx, n, row), table in zip(_sessions(case), x["tables"]):
         for part, rows in ((0, k), (1, v)):
             first = ctx // 16
@@ -445,14 +450,15 @@ def exact(case, seed):
             new = new.view(kvh, -1, 16, hd).transpose(0, 1)  # [page][head][slot][dim]
             e = torch.ceil(torch.log2(new.abs().amax((-1, -2)) / 448.0)).clamp(-15, 7)
             if ctx % 16:
-                e[0] = torch.maximum(e[0], x["exps"][table[first], :, part].double())
+                e[0] = torch.maximum(e[0], torch.log2(scales[table[first], :, part]))
             place = at[part, :, :hd].reshape(-1)
             new = new * 2.0 ** -e[..., None, None]
             if ctx % 16:
                 was = codes[table[first]][:, place].view(kvh, 16, hd)
-                was = was * 2.0 ** (x["exps"][table[first], :, part].double() - e[0])[:, None, None]
+                was = was * (scales[table[first], :, part] / 2.0 ** e[0])[:, None, None]
                 new[0, :, : ctx % 16] = was[:, : ctx % 16]
             page = codes[table[first:]]
             page[:, :, place] = new.reshape(len(table) - first, kvh, 16 * hd)
             codes[table[first:]] = page
-    return dict(got, codes=codes, exponents=None)
+            scales[table[first:], :, part] = 2.0 ** e
+    return dict(got, codes=codes, scales=scales)
