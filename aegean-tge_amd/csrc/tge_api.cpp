@@ -17,9 +17,12 @@
 #include <vector>
 
 #include "../host/plan.hpp"
+#include "../host/plan_e4m3.hpp"
+#include "e4m3_kernels.h"
 #include "tge_common.h"
 #include "tge_error.h"
 #include "tge_kernels.h"
+#include "tge_layer.h"
 
 namespace {
 
@@ -79,6 +82,8 @@ struct tge_kv_pool {
   int bd = 0;               // block width (dims per token of a page block)
   tge::BlockGeom geom{};
   size_t layer_blocks = 0;  // pages * kv_heads
+  size_t layer_bytes = 0;   // the page blocks, then (e4m3) the blocks' scale pairs
+  int device = 0;
   size_t bytes = 0;
 };
 
@@ -171,6 +176,19 @@ struct StepPlan {
   }
 };
 
+// A step on an e4m3 pool: everything that its append and attention launches
+// read is uploaded with the plan, so the calls themselves only launch.
+struct E4m3Plan {
+  tge::plan::E4m3Lists lists;
+  bool built = false;
+  size_t off_tiles = 0, off_items = 0, off_first = 0, off_merges = 0, off_counters = 0;  // in the batch image
+  tge::plan::Scratch part_o, part_ml;
+  ~E4m3Plan() {
+    part_o.release(g_mem);
+    part_ml.release(g_mem);
+  }
+};
+
 }  // namespace
 
 struct tge_batch {
@@ -181,6 +199,7 @@ struct tge_batch {
   // batches depend on it).
   int format = 0, scale_format = 0;
   AttnPlan decode, prefill;
+  E4m3Plan e4;
   // Mixed steps (tge_batch_attention): the decode kernel over the sessions
   // whose rows fit a decode unit, the prefill kernel over the others.
   AttnPlan mix_decode, mix_prefill;
@@ -261,6 +280,12 @@ int tge_kv_v_index(int token, int dim, int format) {
   if (format != TGE_KV_F16 && format != TGE_KV_I8) return -1;
   return tge::v_index(token, dim, format == TGE_KV_F16 ? 2 : 1);
 }
+int tge_kv_e4m3_index(int part, int token, int dim, int block_dims) {
+  if ((part != 0 && part != 1) || token < 0 || token >= TGE_PAGE_TOKENS || dim < 0 || dim >= block_dims ||
+      (block_dims != 64 && block_dims != 128 && block_dims != 256))
+    return -1;
+  return part == 0 ? tge::e4m3_k_index(token, dim) : tge::e4m3_v_index(token, dim, block_dims);
+}
 int tge_kv_scale_index(int token, int block, int head_dim) {
   return tge::scale_index_np(token, block, head_dim / 32);
 }
@@ -273,15 +298,19 @@ int tge_kv_pool_create(const tge_kv_pool_desc* desc, tge_kv_pool** out) {
   const tge_kv_pool_desc& d = *desc;
   if (d.layers <= 0 || d.pages <= 0 || d.kv_heads <= 0)
     return fail(TGE_ERR_INVALID, "kv_pool_create: non-positive size");
-  if (d.format != TGE_KV_F16 && d.format != TGE_KV_I8)
+  if (d.format != TGE_KV_F16 && d.format != TGE_KV_I8 && d.format != TGE_KV_E4M3)
     return fail(TGE_ERR_INVALID, "kv_pool_create: unknown format");
   if (tge::block_dims_for(d.head_dim, d.format) == 0)
     return fail(TGE_ERR_INVALID, d.format == TGE_KV_I8
                                      ? "kv_pool_create: int8 head_dim must be a multiple of 32 up to 256"
+                                 : d.format == TGE_KV_E4M3
+                                     ? "kv_pool_create: e4m3 head_dim must be a multiple of 8 up to 256"
                                      : "kv_pool_create: head_dim must be a multiple of 4 up to 256");
   if (d.format == TGE_KV_I8 && d.scale_format != TGE_SCALE_F16 &&
       d.scale_format != TGE_SCALE_F32)
     return fail(TGE_ERR_INVALID, "kv_pool_create: unknown scale format");
+  if (d.format == TGE_KV_E4M3 && (long long)d.pages * d.kv_heads > INT_MAX)
+    return fail(TGE_ERR_INVALID, "kv_pool_create: pages * kv_heads exceeds int");
   const int s = backend_ready();
   if (s != TGE_OK) return fail(s, "kv_pool_create: backend unavailable");
 
@@ -292,9 +321,11 @@ int tge_kv_pool_create(const tge_kv_pool_desc* desc, tge_kv_pool** out) {
   p->layer_blocks = (size_t)d.pages * d.kv_heads;
   // Kernels address a page block by its 64-bit address (one buffer
   // resource per block), so a layer's array has no 32-bit limit.
-  const size_t layer_bytes = (size_t)p->geom.block_bytes * p->layer_blocks;
-  const size_t total = layer_bytes * d.layers;
-  hipError_t e = hipMalloc(&p->blocks, total);
+  p->layer_bytes = (size_t)p->geom.block_bytes * p->layer_blocks;
+  if (d.format == TGE_KV_E4M3) p->layer_bytes += align_up(p->layer_blocks * sizeof(uint32_t));
+  const size_t total = p->layer_bytes * d.layers;
+  hipError_t e = hipGetDevice(&p->device);
+  if (e == hipSuccess) e = hipMalloc(&p->blocks, total);
   if (e == hipSuccess) e = hipMemset(p->blocks, 0, total);
   if (e != hipSuccess) {
     tge_kv_pool_destroy(p);
@@ -318,12 +349,16 @@ int tge_kv_pool_layer(const tge_kv_pool* p, int layer, tge_kv_layer_view* out) {
   if (!p || !out) return fail(TGE_ERR_INVALID, "kv_pool_layer: null argument");
   if (layer < 0 || layer >= p->desc.layers)
     return fail(TGE_ERR_INVALID, "kv_pool_layer: layer out of range");
-  char* base = static_cast<char*>(p->blocks) + (size_t)p->geom.block_bytes * p->layer_blocks * layer;
+  char* base = static_cast<char*>(p->blocks) + p->layer_bytes * layer;
   const bool i8 = p->desc.format == TGE_KV_I8;
   out->k = base;
   out->v = base + p->geom.v_off();
   out->k_scales = i8 ? base + p->geom.ks_off() : nullptr;
   out->v_scales = i8 ? base + p->geom.vs_off() : nullptr;
+  if (p->desc.format == TGE_KV_E4M3) {
+    out->k_scales = base + (size_t)p->geom.block_bytes * p->layer_blocks;
+    out->v_scales = static_cast<char*>(out->k_scales) + sizeof(uint16_t);
+  }
   out->block_dims = p->bd;
   out->kv_block_bytes = (size_t)p->geom.kv_bytes;
   out->scale_block_bytes = (size_t)p->geom.scale_bytes;
@@ -339,11 +374,18 @@ int tge_kv_copy_page(tge_kv_pool* p, int src_page, int dst_page, void* stream) {
   // A page's blocks are kv_heads consecutive blocks in every layer's array:
   // one strided copy of `layers` rows.
   const size_t row = (size_t)p->geom.block_bytes * p->desc.kv_heads;
-  const size_t pitch = (size_t)p->geom.block_bytes * p->layer_blocks;
+  const size_t pitch = p->layer_bytes;
   char* base = static_cast<char*>(p->blocks);
   TGE_HIP(hipMemcpy2DAsync(base + row * dst_page, pitch, base + row * src_page, pitch, row,
                            (size_t)p->desc.layers, hipMemcpyDeviceToDevice,
                            static_cast<hipStream_t>(stream)));
+  if (p->desc.format == TGE_KV_E4M3) {
+    const size_t pairs = sizeof(uint32_t) * p->desc.kv_heads;
+    base += (size_t)p->geom.block_bytes * p->layer_blocks;
+    TGE_HIP(hipMemcpy2DAsync(base + pairs * dst_page, pitch, base + pairs * src_page, pitch, pairs,
+                             (size_t)p->desc.layers, hipMemcpyDeviceToDevice,
+                             static_cast<hipStream_t>(stream)));
+  }
   return TGE_OK;
 }
 
@@ -484,6 +526,52 @@ int finish_step_plan(tge_batch* b, hipStream_t st) {
   return TGE_OK;
 }
 
+// The e4m3 part of tge_batch_plan: one upload holds
+// [ tables | rows | append tiles | items | wg_first | merges | counters ].
+int plan_e4m3(tge_batch* b, hipStream_t hs) {
+  const tge::plan::Step& st = b->step;
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  TGE_HIP(hipStreamIsCapturing(hs, &cs));
+  if (cs != hipStreamCaptureStatusNone)
+    return fail(TGE_ERR_INVALID,
+                "batch_plan: the stream is capturing (the plan is uploaded from host memory, which a "
+                "graph would replay stale; plan first, then capture the calls)");
+  E4m3Plan& e = b->e4;
+  tge::plan::build_e4m3(st, device_cus() * tge::e4m3_groups_per_cu(st.block_dims), e.lists);
+  const auto& L = e.lists;
+  if ((size_t)L.parts * tge::kE4m3Rows * st.block_dims * sizeof(float) > 0x7fffffffu)
+    return fail(TGE_ERR_CAPACITY, "batch_plan: the step's partial states exceed 2 GiB");
+  const size_t o_rows = align_up(st.tables.size() * sizeof(int));
+  e.off_tiles = align_up(o_rows + st.rows.size() * sizeof(tge::RowRec));
+  e.off_items = align_up(e.off_tiles + L.tiles.size() * sizeof(tge::E4m3Tile));
+  e.off_first = align_up(e.off_items + L.items.size() * sizeof(tge::E4m3Item));
+  e.off_merges = align_up(e.off_first + L.wg_first.size() * sizeof(int));
+  e.off_counters = align_up(e.off_merges + L.merges.size() * sizeof(tge::E4m3Merge));
+  const size_t total = e.off_counters + L.merges.size() * sizeof(int);
+  int s = b->image.upload(g_mem, total, hs, [&](char* h) {
+    auto put = [&](size_t at, const auto& v) {
+      if (!v.empty()) std::memcpy(h + at, v.data(), v.size() * sizeof(v[0]));
+    };
+    put(0, st.tables);
+    put(o_rows, st.rows);
+    put(e.off_tiles, L.tiles);
+    put(e.off_items, L.items);
+    put(e.off_first, L.wg_first);
+    put(e.off_merges, L.merges);
+    if (!L.merges.empty()) std::memset(h + e.off_counters, 0, L.merges.size() * sizeof(int));
+  });
+  if (s != TGE_OK) return s;
+  b->off_tables = 0;
+  b->off_rows = o_rows;
+  const size_t rows = (size_t)std::max(L.parts, 1) * tge::kE4m3Rows;
+  s = e.part_o.reserve(g_mem, rows * st.block_dims * sizeof(float), hs);
+  if (s == TGE_OK) s = e.part_ml.reserve(g_mem, rows * 2 * sizeof(float), hs);
+  if (s != TGE_OK) return s;
+  e.built = true;
+  b->planned = true;
+  return TGE_OK;
+}
+
 }  // namespace
 
 int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* d,
@@ -502,8 +590,11 @@ int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* 
   b->prefill.built = false;
   b->decode.built = false;
   b->mix_built = false;
+  b->small.built = false;
+  b->e4.built = false;
 
   hipStream_t hs = static_cast<hipStream_t>(stream);
+  if (pool->desc.format == TGE_KV_E4M3) return plan_e4m3(b, hs);
   // The step's lists are built on the host first and go up in one copy:
   // [ sessions | tables | rows | append tiles | attention lists | step records |
   // first-batch page ids ]. The attention lists are the decode lists when
@@ -575,6 +666,14 @@ int tge_batch_info(const tge_batch* b, int* rows, int* work_items, int* max_spli
   // Decode figures of the current plan; a plan whose rows exceed a decode
   // unit has none (0, 0).
   const bool dec = b->decode.built;
+  if (b->e4.built) {
+    int most = 1;
+    for (const auto& m : b->e4.lists.merges) most = std::max(most, m.n_parts);
+    if (rows) *rows = (int)b->step.rows.size();
+    if (work_items) *work_items = (int)b->e4.lists.items.size();
+    if (max_splits) *max_splits = most;
+    return TGE_OK;
+  }
   if (rows) *rows = (int)b->step.rows.size();
   if (work_items) *work_items = dec ? (int)b->decode.lists.work.size() : 0;
   if (max_splits) *max_splits = dec ? b->decode.lists.max_splits : 0;
@@ -745,13 +844,213 @@ int run_attention(const tge_batch* b, const tge_kv_pool* p, int layer, const flo
   return TGE_OK;
 }
 
+// What the e4m3 calls ask beyond check_use.
+int check_e4m3(const tge_batch* b, const tge_kv_pool* p, const char* who) {
+  if (p->desc.format != TGE_KV_E4M3 || !b->e4.built)
+    return fail(TGE_ERR_INVALID, std::string(who) + ": needs a TGE_KV_E4M3 pool");
+  int dev = 0;
+  TGE_HIP(hipGetDevice(&dev));
+  if (dev != p->device) return fail(TGE_ERR_INVALID, std::string(who) + ": the pool is on another device");
+  return TGE_OK;
+}
+
+// A row array: its base and stride (elements; 0: `len`, rows without gaps).
+int check_rows(const void* base, long long* stride, long long len, int type, const char* who, const char* name) {
+  if (*stride == 0) *stride = len;
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0)
+    return fail(TGE_ERR_INVALID, std::string(who) + ": " + name + " is not 16-byte aligned");
+  if (*stride < len || *stride % (type == TGE_ROWS_F32 ? 4 : 8) != 0)
+    return fail(TGE_ERR_INVALID, std::string(who) + ": " + name +
+                                     "'s stride must be at least a row and a multiple of 16 bytes");
+  return TGE_OK;
+}
+
+int check_row_type(int type, const char* who) {
+  return type == TGE_ROWS_F32 || type == TGE_ROWS_F16 || type == TGE_ROWS_BF16
+             ? TGE_OK
+             : fail(TGE_ERR_INVALID, std::string(who) + ": unknown row type");
+}
+
+int append_e4m3(const tge_batch* b, tge_kv_pool* p, int layer, const tge_append_rows_args& a, void* stream,
+                const char* who) {
+  int s = check_e4m3(b, p, who);
+  if (s == TGE_OK) s = check_row_type(a.row_type, who);
+  if (s != TGE_OK) return s;
+  if (!a.k || !a.v) return fail(TGE_ERR_INVALID, std::string(who) + ": null k/v");
+  if (b->e4.lists.page_twice)
+    return fail(TGE_ERR_INVALID, std::string(who) + ": two sessions would write into one page");
+  const int hd = b->step.head_dim;
+  const long long kvd = (long long)b->step.kv_heads * hd, qd = (long long)b->step.q_heads * hd;
+  long long ks = a.k_stride, vs = a.v_stride, qs = a.q_stride, os = a.q_out_stride;
+  s = check_rows(a.k, &ks, kvd, a.row_type, who, "k");
+  if (s == TGE_OK) s = check_rows(a.v, &vs, kvd, a.row_type, who, "v");
+  if (s != TGE_OK) return s;
+  const bool rope = a.rope_cos || a.rope_sin;
+  if (rope) {
+    if (!a.rope_cos || !a.rope_sin) return fail(TGE_ERR_INVALID, std::string(who) + ": one rotary table without the other");
+    if (hd % 16 != 0) return fail(TGE_ERR_INVALID, std::string(who) + ": head_dim must be a multiple of 16 to rotate");
+    if (a.q && !a.q_out) return fail(TGE_ERR_INVALID, std::string(who) + ": q without q_out");
+    if (!a.q && a.q_out) return fail(TGE_ERR_INVALID, std::string(who) + ": q_out without q");
+    if (a.q) {
+      s = check_rows(a.q, &qs, qd, a.row_type, who, "q");
+      if (s == TGE_OK) s = check_rows(a.q_out, &os, qd, a.row_type, who, "q_out");
+      if (s != TGE_OK) return s;
+      if (a.q == a.q_out && qs != os)
+        return fail(TGE_ERR_INVALID, std::string(who) + ": q rotated in place needs one stride");
+    }
+    for (const auto& r : b->step.sessions)
+      if (r.ctx + r.n_new > a.rope_positions)
+        return fail(TGE_ERR_INVALID, std::string(who) + ": a position is past the rotary tables");
+  } else if (a.q || a.q_out || a.q_bias || a.k_bias || a.v_bias) {
+    return fail(TGE_ERR_INVALID, std::string(who) + ": q and biases need the rotary tables");
+  }
+  tge_kv_layer_view view{};
+  tge_kv_pool_layer(p, layer, &view);
+  const E4m3Plan& e = b->e4;
+  tge::E4m3Append x{};
+  x.k = a.k;
+  x.v = a.v;
+  x.k_stride = (long)ks;
+  x.v_stride = (long)vs;
+  x.row_type = a.row_type;
+  x.blocks = static_cast<char*>(view.k);
+  x.scales = static_cast<uint32_t*>(view.k_scales);
+  x.tiles = reinterpret_cast<const tge::E4m3Tile*>(b->image.dev + e.off_tiles);
+  x.n_tiles = (int)e.lists.tiles.size();
+  x.kv_heads = b->step.kv_heads;
+  x.dims = hd;
+  x.width = p->bd;
+  x.q = a.q;
+  x.q_out = a.q_out;
+  x.q_stride = (long)qs;
+  x.q_out_stride = (long)os;
+  x.rows = reinterpret_cast<const tge::RowRec*>(b->image.dev + b->off_rows);
+  x.n_rows = (int)b->step.rows.size();
+  x.q_heads = b->step.q_heads;
+  x.q_bias = a.q_bias;
+  x.k_bias = a.k_bias;
+  x.v_bias = a.v_bias;
+  x.rope_cos = a.rope_cos;
+  x.rope_sin = a.rope_sin;
+  x.rope_fma = a.rope_fma ? 1 : 0;
+  TGE_HIP(tge::launch_e4m3_append(x, static_cast<hipStream_t>(stream)));
+  return TGE_OK;
+}
+
+// Checks an attention call and fills its kernel parameters.
+int attention_params_e4m3(const tge_batch* b, const tge_kv_pool* p, int layer, const tge_attention_rows_args& a,
+                          const char* who, tge::E4m3Attn& x) {
+  int s = check_e4m3(b, p, who);
+  if (s == TGE_OK) s = check_row_type(a.row_type, who);
+  if (s != TGE_OK) return s;
+  if (!a.q || !a.out) return fail(TGE_ERR_INVALID, std::string(who) + ": null q/out");
+  if (b->sp_stride > 0)
+    return fail(TGE_ERR_INVALID, std::string(who) + ": no static sparse subset on a TGE_KV_E4M3 pool");
+  const int hd = b->step.head_dim;
+  const long long qd = (long long)b->step.q_heads * hd;
+  long long qs = a.q_stride, os = a.out_stride;
+  s = check_rows(a.q, &qs, qd, a.row_type, who, "q");
+  if (s == TGE_OK) s = check_rows(a.out, &os, qd, a.row_type, who, "out");
+  if (s != TGE_OK) return s;
+  if (!(a.scale >= 0.0f) || std::isinf(a.scale))
+    return fail(TGE_ERR_INVALID, std::string(who) + ": scale must be finite and not negative");
+  tge_kv_layer_view view{};
+  tge_kv_pool_layer(p, layer, &view);
+  const E4m3Plan& e = b->e4;
+  x.blocks = static_cast<const char*>(view.k);
+  x.scales = static_cast<const uint32_t*>(view.k_scales);
+  x.items = reinterpret_cast<const tge::E4m3Item*>(b->image.dev + e.off_items);
+  x.wg_first = reinterpret_cast<const int*>(b->image.dev + e.off_first);
+  x.tables = reinterpret_cast<const int*>(b->image.dev + b->off_tables);
+  x.merges = reinterpret_cast<const tge::E4m3Merge*>(b->image.dev + e.off_merges);
+  x.counters = reinterpret_cast<int*>(b->image.dev + e.off_counters);
+  x.q = a.q;
+  x.out = a.out;
+  x.q_stride = (long)qs;
+  x.out_stride = (long)os;
+  x.row_type = a.row_type;
+  x.kv_heads = b->step.kv_heads;
+  x.group = b->step.group;
+  x.dims = hd;
+  x.scale_log2 = (float)(1.4426950408889634 * (a.scale > 0.0f ? (double)a.scale : 1.0 / std::sqrt((double)hd)));
+  x.part_o = reinterpret_cast<float*>(e.part_o.dev);
+  x.part_ml = reinterpret_cast<float*>(e.part_ml.dev);
+  return TGE_OK;
+}
+
+int attend_e4m3(const tge_batch* b, const tge_kv_pool* p, int layer, const tge_attention_rows_args& a, void* stream,
+                const char* who) {
+  tge::E4m3Attn x{};
+  int s = attention_params_e4m3(b, p, layer, a, who, x);
+  if (s != TGE_OK) return s;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  std::array<hipEvent_t, 3>* ev = nullptr;
+  s = profile_events(const_cast<tge_batch*>(b), &ev);
+  if (s != TGE_OK) return s;
+  if (ev) TGE_HIP(hipEventRecord((*ev)[0], st));
+  TGE_HIP(tge::launch_e4m3_attention(p->bd, b->e4.lists.groups, x, st));
+  if (ev) {
+    TGE_HIP(hipEventRecord((*ev)[1], st));
+    TGE_HIP(hipEventRecord((*ev)[2], st));
+  }
+  return TGE_OK;
+}
+
+// The fp32 entry points on an e4m3 pool.
+int attend_e4m3_f32(const tge_batch* b, const tge_kv_pool* p, int layer, const float* q, float* out, void* stream,
+                    const char* who) {
+  tge_attention_rows_args a{};
+  a.q = q;
+  a.out = out;
+  return attend_e4m3(b, p, layer, a, stream, who);
+}
+
+int append_e4m3_f32(const tge_batch* b, tge_kv_pool* p, int layer, const float* k, const float* v, void* stream,
+                    const char* who) {
+  tge_append_rows_args a{};
+  a.k = k;
+  a.v = v;
+  return append_e4m3(b, p, layer, a, stream, who);
+}
+
 }  // namespace
+
+int tge_kv_append_rows(const tge_batch* b, tge_kv_pool* p, int layer, const tge_append_rows_args* a, void* stream) {
+  const int s = check_use(b, p, layer, "kv_append_rows");
+  if (s != TGE_OK) return s;
+  if (!a) return fail(TGE_ERR_INVALID, "kv_append_rows: null argument");
+  return append_e4m3(b, p, layer, *a, stream, "kv_append_rows");
+}
+
+int tge_attention_rows(const tge_batch* b, const tge_kv_pool* p, int layer, const tge_attention_rows_args* a,
+                       void* stream) {
+  const int s = check_use(b, p, layer, "attention_rows");
+  if (s != TGE_OK) return s;
+  if (!a) return fail(TGE_ERR_INVALID, "attention_rows: null argument");
+  return attend_e4m3(b, p, layer, *a, stream, "attention_rows");
+}
+
+}  // extern "C"
+
+// append + attention; every refusal of either comes before the first launch.
+int tge::layer_rows(const tge_batch* b, tge_kv_pool* p, int layer, const tge_append_rows_args& store,
+                    const tge_attention_rows_args& attend, void* stream) {
+  int s = check_use(b, p, layer, "layer_rows");
+  tge::E4m3Attn x{};
+  if (s == TGE_OK) s = attention_params_e4m3(b, p, layer, attend, "layer_rows", x);
+  if (s == TGE_OK) s = append_e4m3(b, p, layer, store, stream, "layer_rows");
+  if (s == TGE_OK) s = attend_e4m3(b, p, layer, attend, stream, "layer_rows");
+  return s;
+}
+
+extern "C" {
 
 int tge_kv_append(const tge_batch* b, tge_kv_pool* p, int layer, const float* k,
                   const float* v, void* stream) {
   int s = check_use(b, p, layer, "kv_append");
   if (s != TGE_OK) return s;
   if (!k || !v) return fail(TGE_ERR_INVALID, "kv_append: null k/v");
+  if (p->desc.format == TGE_KV_E4M3) return append_e4m3_f32(b, p, layer, k, v, stream, "kv_append");
   tge_kv_layer_view view{};
   tge_kv_pool_layer(p, layer, &view);
   tge::AppendParams a{};
@@ -788,6 +1087,21 @@ int tge_kv_append_rope(const tge_batch* b, tge_kv_pool* p, int layer,
   for (const auto& row : b->step.rows) max_pos = std::max(max_pos, row.pos);
   if (max_pos >= r->rope_positions)
     return fail(TGE_ERR_INVALID, "kv_append_rope: a position is past the rotary tables");
+  if (p->desc.format == TGE_KV_E4M3) {
+    tge_append_rows_args x{};
+    x.k = r->k;
+    x.v = r->v;
+    x.q = r->q;
+    x.q_out = r->q ? r->q_out : nullptr;
+    x.q_bias = r->q_bias;
+    x.k_bias = r->k_bias;
+    x.v_bias = r->v_bias;
+    x.rope_cos = r->rope_cos;
+    x.rope_sin = r->rope_sin;
+    x.rope_positions = r->rope_positions;
+    x.rope_fma = r->rope_fma;
+    return append_e4m3(b, p, layer, x, stream, "kv_append_rope");
+  }
   tge_kv_layer_view view{};
   tge_kv_pool_layer(p, layer, &view);
   tge::AppendParams a{};
@@ -842,6 +1156,11 @@ int tge_decode_attention(const tge_batch* b, const tge_kv_pool* p, int layer,
   int s = check_use(b, p, layer, "decode_attention");
   if (s != TGE_OK) return s;
   if (!q || !out) return fail(TGE_ERR_INVALID, "decode_attention: null q/out");
+  if (p->desc.format == TGE_KV_E4M3) {
+    if (b->step.max_rows > tge::kMaxRows)
+      return fail(TGE_ERR_INVALID, "decode_attention: n_new * group exceeds a decode unit (64 rows)");
+    return attend_e4m3_f32(b, p, layer, q, out, stream, "decode_attention");
+  }
   if (!b->decode.built)
     return fail(TGE_ERR_INVALID, "decode_attention: n_new * group exceeds a decode unit (64 rows, 48 at head_dim > 128)");
   if (b->decode.sparse != (b->sp_stride > 0)) {
@@ -858,6 +1177,17 @@ int tge_decode_step(const tge_batch* b, tge_kv_pool* p, int layer, const float* 
   int s = check_use(b, p, layer, "decode_step");
   if (s != TGE_OK) return s;
   if (!q || !k || !v || !out) return fail(TGE_ERR_INVALID, "decode_step: null q/k/v/out");
+  if (p->desc.format == TGE_KV_E4M3) {
+    if (b->step.max_rows > tge::kMaxRows)
+      return fail(TGE_ERR_INVALID, "decode_step: n_new * group exceeds a decode unit (64 rows)");
+    tge_append_rows_args store{};
+    store.k = k;
+    store.v = v;
+    tge_attention_rows_args attend{};
+    attend.q = q;
+    attend.out = out;
+    return tge::layer_rows(b, p, layer, store, attend, stream);
+  }
   if (!b->decode.built)
     return fail(TGE_ERR_INVALID, "decode_step: n_new * group exceeds a decode unit (64 rows, 48 at head_dim > 128)");
   if (b->sp_stride > 0 && !one_kernel_step(b)) {
@@ -920,6 +1250,7 @@ int tge_prefill_attention(const tge_batch* b, const tge_kv_pool* p, int layer,
   int s = check_use(b, p, layer, "prefill_attention");
   if (s != TGE_OK) return s;
   if (!q || !out) return fail(TGE_ERR_INVALID, "prefill_attention: null q/out");
+  if (p->desc.format == TGE_KV_E4M3) return attend_e4m3_f32(b, p, layer, q, out, stream, "prefill_attention");
   // The prefill lists are built on first use after each plan (decode-only
   // steps never pay for them) and reused by every layer.
   tge_batch* mb = const_cast<tge_batch*>(b);
@@ -938,6 +1269,7 @@ int tge_batch_attention(const tge_batch* b, const tge_kv_pool* p, int layer, con
   int s = check_use(b, p, layer, "batch_attention");
   if (s != TGE_OK) return s;
   if (!q || !out) return fail(TGE_ERR_INVALID, "batch_attention: null q/out");
+  if (p->desc.format == TGE_KV_E4M3) return attend_e4m3_f32(b, p, layer, q, out, stream, "batch_attention");
   tge_batch* mb = const_cast<tge_batch*>(b);
   int n_dec = 0, n_pf = 0;
   for (const auto& sr : b->step.sessions) (tge::plan::decode_session(b->step, sr) ? n_dec : n_pf)++;
@@ -1036,6 +1368,8 @@ int tge_decode_attention_static(const tge_batch_desc* d, const tge_kv_pool* p, i
   if (!d || !p || !q || !out) return fail(TGE_ERR_INVALID, "decode_attention_static: null argument");
   if (layer < 0 || layer >= p->desc.layers)
     return fail(TGE_ERR_INVALID, "decode_attention_static: layer out of range");
+  if (p->desc.format == TGE_KV_E4M3)
+    return fail(TGE_ERR_INVALID, "decode_attention_static: not for a TGE_KV_E4M3 pool");
   int s = backend_ready();
   if (s != TGE_OK) return fail(s, "decode_attention_static: backend unavailable");
   {
@@ -1150,6 +1484,8 @@ int tge_attention_group(const tge_attention_group_args* a, void* stream) {
     return fail(TGE_ERR_INVALID, "attention_group: layer out of range");
   if (a->kv_head < 0 || a->kv_head >= p->desc.kv_heads)
     return fail(TGE_ERR_INVALID, "attention_group: kv_head out of range");
+  if (p->desc.format == TGE_KV_E4M3)
+    return fail(TGE_ERR_INVALID, "attention_group: not for a TGE_KV_E4M3 pool");
   if (!a->page_ids || !a->queries || !a->maxima || !a->sums || !a->accumulators)
     return fail(TGE_ERR_INVALID, "attention_group: null pointer");
   if (a->first < 0 || a->count < 0)
@@ -1195,9 +1531,28 @@ int tge_kv_gather(const tge_batch* b, const tge_kv_pool* p, int layer, int sessi
     return fail(TGE_ERR_INVALID, "kv_gather: count beyond the session's positions");
   if (!k_rows || !v_rows) return fail(TGE_ERR_INVALID, "kv_gather: null rows");
   const bool i8 = p->desc.format == TGE_KV_I8;
-  if (i8 && (!k_scales || !v_scales)) return fail(TGE_ERR_INVALID, "kv_gather: null scales");
+  const bool e4m3 = p->desc.format == TGE_KV_E4M3;
+  if ((i8 || e4m3) && (!k_scales || !v_scales)) return fail(TGE_ERR_INVALID, "kv_gather: null scales");
   tge_kv_layer_view view{};
   tge_kv_pool_layer(p, layer, &view);
+  if (e4m3) {
+    s = check_e4m3(b, p, "kv_gather");
+    if (s != TGE_OK) return s;
+    tge::E4m3Gather x{};
+    x.blocks = static_cast<const char*>(view.k);
+    x.scales = static_cast<const uint32_t*>(view.k_scales);
+    x.table = reinterpret_cast<const int*>(b->image.dev + b->off_tables) + sr.table_off;
+    x.count = count;
+    x.kv_heads = b->step.kv_heads;
+    x.dims = b->step.head_dim;
+    x.width = p->bd;
+    x.k_rows = static_cast<uint8_t*>(k_rows);
+    x.v_rows = static_cast<uint8_t*>(v_rows);
+    x.k_scales = static_cast<uint16_t*>(k_scales);
+    x.v_scales = static_cast<uint16_t*>(v_scales);
+    TGE_HIP(tge::launch_e4m3_gather(x, static_cast<hipStream_t>(stream)));
+    return TGE_OK;
+  }
   tge::GatherParams g{};
   g.pool = view.k;
   g.geom = p->geom;

@@ -9,7 +9,7 @@
 
 namespace tge {
 
-enum Format { kF16 = 1, kI8 = 2 };
+enum Format { kF16 = 1, kI8 = 2, kE4M3 = 4 };
 
 // ---------------------------------------------------------------------------
 // Page blocks. One layer's pool is one array of pages*kv_heads page blocks;
@@ -31,19 +31,20 @@ struct BlockGeom {
 // stored in 64-dim blocks, up to 128 in 128-dim blocks, up to 256 in
 // 256-dim blocks, the dims from head_dim on holding zeros (so scores and
 // values are those of the head's own dims). A head size must be a positive
-// multiple of 4 (int8: of 32, the quantizer's block) of at most 256; 0 for
-// any other. Every kernel reads and writes the head's own dims of q, k, v
+// multiple of 4 (int8: of 32, the quantizer's block; e4m3: of 8) of at most
+// 256; 0 for any other. Every kernel reads and writes the head's own dims of q, k, v
 // and out in 16-byte runs of 4 that lie wholly inside or outside them (the
 // rows stay 16-byte aligned).
 __host__ __device__ inline int block_dims_for(int head_dim, int format) {
-  if (head_dim <= 0 || head_dim > 256 || head_dim % (format == kI8 ? 32 : 4) != 0) return 0;
+  if (head_dim <= 0 || head_dim > 256 || head_dim % (format == kI8 ? 32 : format == kE4M3 ? 8 : 4) != 0)
+    return 0;
   return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
 }
 
 __host__ __device__ inline BlockGeom block_geom(int format, int head_dim, int scale_f32) {
   BlockGeom g;
   g.kv_bytes = 16 * head_dim * (format == kF16 ? 2 : 1);
-  g.scale_bytes = format == kF16 ? 0 : 16 * (head_dim / 32) * (scale_f32 ? 4 : 2);
+  g.scale_bytes = format != kI8 ? 0 : 16 * (head_dim / 32) * (scale_f32 ? 4 : 2);
   g.block_bytes = 2 * g.kv_bytes + 2 * g.scale_bytes;
   return g;
 }

@@ -2,7 +2,7 @@
 // driver. See include/tge_amd/qwen2_kv.hpp and include/tge_kv.h.
 #include "tge_amd/qwen2_kv.hpp"
 
-#include "../csrc/tge_error.h"
+#include "qwen2_kv_handles.hpp"
 
 #include <algorithm>
 #include <functional>
@@ -11,21 +11,6 @@
 #include <string>
 
 namespace tge::models {
-namespace {
-
-// A HIP/ABI failure below the driver: carries the C status.
-struct StatusError : std::runtime_error {
-  int status;
-  StatusError(int s, const std::string& what) : std::runtime_error(what), status(s) {}
-};
-
-void check(int status, const char* who) {
-  if (status != TGE_OK) {
-    throw StatusError(status, std::string(who) + ": " + tge_last_error());
-  }
-}
-
-}  // namespace
 
 Qwen2KvPath::Qwen2KvPath(const Qwen2KvConfig& config) : config_(config) {
   if (config_.layers <= 0 || config_.q_heads <= 0 || config_.kv_heads <= 0 ||
@@ -447,46 +432,6 @@ void Qwen2KvPath::reset_cache() {
 // ---------------------------------------------------------------------------
 // C wrappers
 // ---------------------------------------------------------------------------
-namespace {
-
-template <typename F>
-int guarded(F&& f) {
-  try {
-    f();
-    return TGE_OK;
-  } catch (const tge::models::StatusError& e) {
-    tge::set_last_error(e.what());
-    return e.status;
-  } catch (const std::invalid_argument& e) {
-    tge::set_last_error(e.what());
-    return TGE_ERR_INVALID;
-  } catch (const std::runtime_error& e) {
-    tge::set_last_error(e.what());
-    return TGE_ERR_RUNTIME;
-  } catch (const std::bad_alloc&) {
-    tge::set_last_error("out of host memory");
-    return TGE_ERR_CAPACITY;
-  }
-}
-
-}  // namespace
-
-// A table handle either owns its BlockTable or views the one a driver owns.
-struct tge_block_table {
-  std::unique_ptr<tge::models::BlockTable> owned;
-  tge::models::BlockTable* table;
-  tge_block_table(int blocks, int tokens)
-      : owned(std::make_unique<tge::models::BlockTable>(blocks, tokens)), table(owned.get()) {}
-  explicit tge_block_table(tge::models::BlockTable* view) : table(view) {}
-};
-
-struct tge_qwen2_kv {
-  tge::models::Qwen2KvPath impl;
-  tge_block_table table_view;
-  explicit tge_qwen2_kv(const tge::models::Qwen2KvConfig& c)
-      : impl(c), table_view(&impl.mutable_table()) {}
-};
-
 extern "C" {
 
 int tge_block_table_create(int blocks, int block_tokens, tge_block_table** out) {

@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(HERE, "libtge_kv.so")
 
 PAGE_TOKENS = 16
 OK, ERR_INVALID, ERR_RUNTIME, ERR_UNAVAILABLE, ERR_DEVICE, ERR_CAPACITY = 0, -1, -2, -3, -4, -5
-KV_F16, KV_I8 = 1, 2
+KV_F16, KV_I8, KV_E4M3 = 1, 2, 4
+ROWS_F32, ROWS_F16, ROWS_BF16 = 0, 1, 2
 SCALE_F16, SCALE_F32 = 0, 1
 
 _lib = None
@@ -83,6 +84,37 @@ def rope_args(k, v, rope_cos, rope_sin, positions, q=None, q_out=None, q_bias=No
                           ptr(v_bias), ptr(rope_cos), ptr(rope_sin), int(positions), int(bool(fma)))
 
 
+class AppendRowsArgs(C.Structure):
+    _fields_ = [("row_type", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_longlong),
+                ("v_stride", C.c_longlong), ("q", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_longlong),
+                ("q_out_stride", C.c_longlong), ("q_bias", C.c_void_p), ("k_bias", C.c_void_p),
+                ("v_bias", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+                ("rope_positions", C.c_int), ("rope_fma", C.c_int)]
+
+
+class AttentionRowsArgs(C.Structure):
+    _fields_ = [("row_type", C.c_int), ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_longlong),
+                ("out_stride", C.c_longlong), ("scale", C.c_float)]
+
+
+def _address(a):
+    return a if a is None or isinstance(a, int) else a.ptr
+
+
+def append_rows_args(row_type, k, v, k_stride=0, v_stride=0, q=None, q_out=None, q_stride=0, q_out_stride=0,
+                     q_bias=None, k_bias=None, v_bias=None, rope_cos=None, rope_sin=None, rope_positions=0, fma=True):
+    """tge_append_rows_args from DeviceArrays or device addresses; strides in elements (0: dense)."""
+    return AppendRowsArgs(int(row_type), _address(k), _address(v), int(k_stride), int(v_stride), _address(q),
+                          _address(q_out), int(q_stride), int(q_out_stride), _address(q_bias), _address(k_bias),
+                          _address(v_bias), _address(rope_cos), _address(rope_sin), int(rope_positions),
+                          int(bool(fma)))
+
+
+def attention_rows_args(row_type, q, out, q_stride=0, out_stride=0, scale=0.0):
+    """tge_attention_rows_args from DeviceArrays or device addresses (scale 0: 1/sqrt(head_dim))."""
+    return AttentionRowsArgs(int(row_type), _address(q), _address(out), int(q_stride), int(out_stride), float(scale))
+
+
 def rope_tables(head_dim, positions, theta=10000.0, attn_factor=1.0, factors=None):
     """Host rotary tables (tge_rope_tables): cos, sin as [positions][head_dim/2]."""
     half = head_dim // 2
@@ -116,6 +148,10 @@ SIGNATURES = [
     ("tge_kv_k_index", _I, [_I, _I, _I]),
     ("tge_kv_v_index", _I, [_I, _I, _I]),
     ("tge_kv_scale_index", _I, [_I, _I, _I]),
+    ("tge_kv_e4m3_index", _I, [_I, _I, _I, _I]),
+    ("tge_kv_append_rows", _I, [_VP, _VP, _I, C.POINTER(AppendRowsArgs), _VP]),
+    ("tge_attention_rows", _I, [_VP, _VP, _I, C.POINTER(AttentionRowsArgs), _VP]),
+    ("tge_qwen2_kv_layer_rows", _I, [_VP, _I, C.POINTER(AppendRowsArgs), C.POINTER(AttentionRowsArgs), _VP]),
     ("tge_batch_create", _I, [C.POINTER(_VP)]),
     ("tge_batch_destroy", None, [_VP]),
     ("tge_batch_plan", _I, [_VP, _VP, C.POINTER(BatchDesc), _VP]),
@@ -554,6 +590,14 @@ class Batch:
         check(lib().tge_kv_append_rope(self.h, pool.h, layer, C.byref(args), stream),
               "kv_append_rope")
 
+    def append_rows(self, pool, layer, args, stream=None):
+        """tge_kv_append_rows with an AppendRowsArgs (see append_rows_args)."""
+        check(lib().tge_kv_append_rows(self.h, pool.h, layer, C.byref(args), stream), "kv_append_rows")
+
+    def attention_rows(self, pool, layer, args, stream=None):
+        """tge_attention_rows with an AttentionRowsArgs (see attention_rows_args)."""
+        check(lib().tge_attention_rows(self.h, pool.h, layer, C.byref(args), stream), "attention_rows")
+
     def decode(self, pool, layer, q, out, stream=None):
         check(lib().tge_decode_attention(self.h, pool.h, layer, q.ptr, out.ptr, stream),
               "decode_attention")
@@ -588,7 +632,8 @@ class Batch:
               "prefill_attention")
 
     def gather(self, pool, layer, session, count):
-        """Positions [0, count) of a session as flat rows (codes/bits, scales)."""
+        """Positions [0, count) of a session as flat rows (codes/bits, scales);
+        e4m3: uint8 codes and the blocks' scales (bf16 bits, [pages][kv_heads])."""
         kv_dim = pool.kv_heads * pool.head_dim
         et = np.uint16 if pool.format == KV_F16 else np.int8
         k = DeviceArray((count, kv_dim), et)
@@ -598,6 +643,10 @@ class Batch:
             st = np.float32 if pool.scale_format == SCALE_F32 else np.uint16
             ks = DeviceArray((count, kv_dim // 32), st)
             vs = DeviceArray((count, kv_dim // 32), st)
+        if pool.format == KV_E4M3:
+            k.dtype = v.dtype = np.dtype(np.uint8)
+            ks = DeviceArray((-(-count // PAGE_TOKENS), pool.kv_heads), np.uint16)
+            vs = DeviceArray((-(-count // PAGE_TOKENS), pool.kv_heads), np.uint16)
         check(lib().tge_kv_gather(self.h, pool.h, layer, session, count, k.ptr, v.ptr,
                                   ks.ptr if ks else None, vs.ptr if vs else None, None),
               "kv_gather")
@@ -650,6 +699,10 @@ class Qwen2KvPath:
     def layer_rope(self, layer, args, out):
         """layer() with bias + RoPE fused into the append; attention reads args.q_out."""
         check(lib().tge_qwen2_kv_layer_rope(self.h, layer, C.byref(args), out.ptr, None), "layer")
+
+    def layer_rows(self, layer, store, attend):
+        """tge_kv_append_rows, then tge_attention_rows (e4m3 caches)."""
+        check(lib().tge_qwen2_kv_layer_rows(self.h, layer, C.byref(store), C.byref(attend), None), "layer")
 
     def store(self, layer, k, v):
         """Append-only (cache priming); k/v are DeviceArrays or raw device addresses."""

@@ -81,6 +81,12 @@ class Qwen2KvPath {
   void layer_rope(int layer, const tge_rope_append_args& args, float* out,
                   void* stream = nullptr);
 
+  // Rows of fp32, f16 or bf16 with strides (tge_kv_append_rows, then
+  // tge_attention_rows): TGE_KV_E4M3 caches. With rotation attend.q is
+  // normally store.q_out.
+  void layer_rows(int layer, const tge_append_rows_args& store,
+                  const tge_attention_rows_args& attend, void* stream = nullptr);
+
   // Store this step's K/V rows for `layer` without attending: the cache-
   // priming path (prime_cache_from_table, qwen2.hpp:283-288 and
   // qwen2.cpp:1973-2026, copies rows into a slot with no recompute).

@@ -53,8 +53,13 @@ enum tge_status {
 
 enum tge_kv_format {
   TGE_KV_F16 = 1, /* IEEE half bits, the reference's float_to_half recipe */
-  TGE_KV_I8 = 2   /* int8 codes, one scale per 32 values (store_kv_q8) */
+  TGE_KV_I8 = 2,  /* int8 codes, one scale per 32 values (store_kv_q8) */
+  TGE_KV_E4M3 = 4 /* OCP e4m3 codes, one power of two for the K codes and one
+                     for the V codes of a page's KV head */
 };
+
+/* Element type of the rows of tge_kv_append_rows and tge_attention_rows. */
+enum tge_row_type { TGE_ROWS_F32 = 0, TGE_ROWS_F16 = 1, TGE_ROWS_BF16 = 2 };
 
 enum tge_scale_format {
   TGE_SCALE_F16 = 0, /* scale stored as float_to_half(fp32 scale) */
@@ -84,12 +89,15 @@ const char* tge_backend_arch(void);
  *   K part, then V part: 16 * W elements each (f16 bits or int8 codes)
  *   I8 only, K scales, then V scales: 16 * W/32 scales each (f16 bits or
  *   fp32)
+ *   E4M3: 16 * W codes each, no scales in the block; the layer's blocks are
+ *   followed by a bf16 pair for each block in block order (tge_kv_append_rows)
  * Block (page, kv_head) of a layer is block number page*kv_heads + kv_head.
  * Element (token t, dim d) of a block's part sits at:
  *   K: tge_kv_k_index(t, d, format)  V: tge_kv_v_index(t, d, format)
  *   scale of (t, block b = d/32): tge_kv_scale_index(t, b, W)
- * head_dim: a multiple of 4 up to 256 (F16) or of 32 up to 256 (I8, whose
- * scales cover 32-dim blocks). The reference takes any head_dim > 0
+ *   E4M3, K and V: tge_kv_e4m3_index(part, t, d, W)
+ * head_dim: a multiple of 4 up to 256 (F16), of 8 (E4M3) or of 32 up to 256
+ * (I8, whose scales cover 32-dim blocks). The reference takes any head_dim > 0
  * (attention_scalar.cpp:11-14; int8 % 32, qwen2.cpp:406-409); heads wider
  * than 256 are not supported here. q, k, v and out rows always have the
  * model's head_dim.
@@ -110,10 +118,11 @@ typedef struct {
 typedef struct {
   void* k;        /* device, K part of block 0 (the layer's base address) */
   void* v;        /* V part of block 0 */
-  void* k_scales; /* NULL for F16 */
+  void* k_scales; /* NULL for F16; E4M3: the K scale of block 0, block n's
+                     4 * n bytes further on */
   void* v_scales;
   size_t kv_block_bytes;    /* bytes of one K (or V) part */
-  size_t scale_block_bytes; /* bytes of one scale part (0 for F16) */
+  size_t scale_block_bytes; /* bytes of one scale part (0 for F16 and E4M3) */
   size_t block_bytes;       /* bytes of a whole page block: the block stride */
   int block_dims;           /* the block width W (64, 128 or 256) */
 } tge_kv_layer_view;
@@ -146,6 +155,13 @@ int tge_kv_copy_page(tge_kv_pool* pool, int src_page, int dst_page, void* stream
 int tge_kv_k_index(int token, int dim, int format);
 int tge_kv_v_index(int token, int dim, int format);
 int tge_kv_scale_index(int token, int block, int head_dim);
+
+/* The same for an E4M3 block's K part (part 0) or V part (part 1), in blocks
+ * of width W = 64, 128 or 256; -1 for arguments outside them:
+ *   K: lane = ((d/16)&3)*16 + t,  j = (d/64)*16 + (d&15)
+ *   V: lane = (t/4)*16 + (d&15),  j = ((d/16)&1)*(W/8) + (d/32)*4 + (t&3)
+ *   index = (j/16)*1024 + lane*16 + j%16 */
+int tge_kv_e4m3_index(int part, int token, int dim, int block_dims);
 
 /* ---------------------------------------------------------------------------
  * Batch: the sessions one step works on. A plan is built once per step on the
@@ -327,12 +343,86 @@ int tge_prefill_attention(const tge_batch* batch, const tge_kv_pool* pool,
 int tge_batch_attention(const tge_batch* batch, const tge_kv_pool* pool,
                         int layer, const float* q, float* out, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The e4m3 cache (TGE_KV_E4M3) and rows in 16 bits. No counterpart in the
+ * reference. A block's 16 tokens hold OCP e4m3 codes; its K codes share one
+ * power of two, its V codes another (bf16, 2^e with -15 <= e <= 7), so a
+ * stored value is code * 2^e and every stored value is also an f16 value.
+ *
+ * The two calls below take rows of fp32, f16 or bf16 with a stride, such as
+ * slices of one projection's output: `*_stride` elements lie between rows (0:
+ * none lie between them). Bases are 16-byte aligned and strides multiples of
+ * 16 bytes. The fp32 calls on such a pool (tge_kv_append, tge_kv_append_rope,
+ * tge_decode_attention, tge_decode_step, tge_prefill_attention,
+ * tge_batch_attention, the driver) are the same kernels with fp32 rows.
+ * tge_decode_attention_static, tge_attention_group and a static sparse subset
+ * are refused on such a pool (TGE_ERR_INVALID), and so are these two calls on
+ * any other pool, on a pool of another device than the current one, and
+ * tge_batch_plan on a stream that is capturing. The calls themselves launch
+ * one kernel each and may be captured; a captured call stays valid until its
+ * batch is planned again or destroyed. The plan holds the workspace: calls on
+ * one batch must not overlap on the device (two streams, or two graphs).
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int row_type;        /* enum tge_row_type of k, v, q and q_out */
+  const void* k;       /* device [rows][kv_heads*head_dim] */
+  const void* v;
+  long long k_stride;
+  long long v_stride;
+  /* With rope_cos and rope_sin (both or neither), bias and rotation come
+   * before the store, as in tge_kv_append_rope, in fp32: x + bias, NeoX
+   * halves, head_dim a multiple of 16. q (or NULL) is rotated into q_out,
+   * rounded once to row_type; q_out may be q with the same stride. Without the
+   * tables q, q_out and the biases must be NULL. */
+  const void* q;       /* device [rows][q_heads*head_dim] */
+  void* q_out;
+  long long q_stride;
+  long long q_out_stride;
+  const float* q_bias; /* device, fp32, each may be NULL */
+  const float* k_bias;
+  const float* v_bias;
+  const float* rope_cos; /* device [rope_positions][head_dim/2] */
+  const float* rope_sin;
+  int rope_positions;
+  int rope_fma;        /* roundings of the rotation, as in tge_kv_append_rope */
+} tge_append_rows_args;
+
+/* Store the step's new rows. Per block that receives some: e is the smallest
+ * exponent with max|x| <= 448 * 2^e over the block's new rows, at least -15, at
+ * most 7, and, where the block holds rows of positions before the step, not
+ * below their exponent. A value is stored as the code nearest x * 2^-e (ties to
+ * even), out of range as the largest code, a NaN as zero (stored values are
+ * finite, so no masked position can reach a row); older codes are re-encoded
+ * where e grew. The page's slots behind the last new row are cleared: rows
+ * that an earlier step stored there (rejected drafts) are gone. Two sessions
+ * that write into one page are refused (TGE_ERR_INVALID). */
+int tge_kv_append_rows(const tge_batch* batch, tge_kv_pool* pool, int layer,
+                       const tge_append_rows_args* args, void* stream);
+
+typedef struct {
+  int row_type;   /* enum tge_row_type of q and out */
+  const void* q;  /* device [rows][q_heads*head_dim] */
+  void* out;      /* only the plan's rows are written */
+  long long q_stride;
+  long long out_stride;
+  float scale;    /* of the scores; 0: 1/sqrt(head_dim) */
+} tge_attention_rows_args;
+
+/* Attention of every new token of the batch over its session's positions 0 ..
+ * its own, any mix of decoding, verifying and prompt sessions in one launch.
+ * q is scaled and rounded to f16 once, softmax weights are f16, sums and
+ * accumulators fp32, out is rounded once. A row of NaN gives NaN and touches no
+ * other row. The same inputs give the same bits on every run. */
+int tge_attention_rows(const tge_batch* batch, const tge_kv_pool* pool, int layer,
+                       const tge_attention_rows_args* args, void* stream);
+
 /*
  * Device gather of one session's positions [0, count) back to the flat
  * row-major layout of the reference cache (gather_blocks_row_major,
  * kv_block_layout.hpp:64-84, applied per element): k_rows/v_rows receive
  * [count][kv_heads*head_dim] elements (f16 bits or int8 codes), scales
- * [count][kv_heads*head_dim/32] (I8 only; may be NULL otherwise).
+ * [count][kv_heads*head_dim/32] (I8; may be NULL for F16). E4M3: codes, and
+ * the blocks' scales as bf16 bits, [ceil(count/16)][kv_heads].
  */
 int tge_kv_gather(const tge_batch* batch, const tge_kv_pool* pool, int layer,
                   int session, int count, void* k_rows, void* v_rows,
@@ -498,6 +588,11 @@ int tge_qwen2_kv_layer(tge_qwen2_kv* model, int layer, const float* q,
 int tge_qwen2_kv_layer_rope(tge_qwen2_kv* model, int layer,
                             const tge_rope_append_args* args, float* out,
                             void* stream);
+/* tge_kv_append_rows, then tge_attention_rows, of the step (E4M3 pools): rows
+ * of 16 bits. With rotation attend->q is normally store->q_out. */
+int tge_qwen2_kv_layer_rows(tge_qwen2_kv* model, int layer,
+                            const tge_append_rows_args* store,
+                            const tge_attention_rows_args* attend, void* stream);
 /* Store the step's K/V rows for `layer` without attending: cache priming
  * (prime_cache_from_table, qwen2.hpp:283-288). */
 int tge_qwen2_kv_store(tge_qwen2_kv* model, int layer, const float* k,
