@@ -50,7 +50,7 @@ template <int W>
 struct E4m3Shared {
   alignas(16) char ring[E4m3Cfg<W>::RING];  // at a tile's end: the waves' accumulators
   int ids[kE4m3ItemPages];                  // the item's pages: block numbers
-  uint32_t scales[kE4m3ItemPages];          // and their scale pairs
+  alignas(8) uint32_t scales[kE4m3ItemPages];  // and their scale pairs
   long out_at[kE4m3Rows];                   // element offset of each row in out
   float ml[2][4][32];                       // per wave: base, sum
   float sum[kE4m3Rows];
@@ -121,31 +121,78 @@ __device__ __forceinline__ void fetch_block(char* slot, const char* blocks, int 
 #endif
 }
 
+// The codes of 32 tokens (two blocks) in a lane's operand order, and the
+// blocks' scale pairs.
+template <int W>
+struct E4m3Codes {
+  static constexpr int KS = W / 32;  // K pieces of 16 dims (two operands each)
+  static constexpr int NT = W / 32;  // 32-dim output tiles
+  u32x4_t k[KS];
+  uint32_t v[2][2][NT];  // [block][tokens 4h.. | 8 + 4h..][dims 32i + c]
+  uint32_t sa, sb;
+
+  // From the two blocks at `slot`, every read issued before any is waited for.
+  __device__ __forceinline__ void read(const char* slot, const uint32_t* scales, int lane) {
+    constexpr int BLOCK = E4m3Cfg<W>::BLOCK;
+    const int c = lane & 31, h = lane >> 5;
+    const u32x2_t s = *reinterpret_cast<const u32x2_t*>(scales);
+    const char* kp = slot + (c >> 4) * BLOCK + h * 256 + (c & 15) * 16;
+#pragma unroll
+    for (int u = 0; u < KS; ++u) k[u] = *reinterpret_cast<const u32x4_t*>(kp + u * 512);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const char* vp = slot + b * BLOCK + 16 * W + (h * 16 + (c & 15)) * 16;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (W == 64) {
+          const u32x2_t x = *reinterpret_cast<const u32x2_t*>(vp + (c >> 4) * 8 + t * 512);
+          v[b][t][0] = x[0];
+          v[b][t][1] = x[1];
+        } else {
+#pragma unroll
+          for (int i = 0; i < NT; i += 4) {
+            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(vp + (c >> 4) * (8 * W) + i * 256 + t * 512);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[b][t][i + e] = x[e];
+          }
+        }
+      }
+    }
+    sa = s[0];
+    sb = s[1];
+  }
+};
+
 // A wave's rows against pages.
 template <int W>
 struct E4m3Rows {
-  static constexpr int KS = W / 32;  // pieces of 16 dims a lane holds (two operands each)
-  static constexpr int NT = W / 32;  // 32-dim output tiles
-  half8_t q[KS][2];                  // row c, dims 32u + 16h + 8x ..
+  static constexpr int KS = E4m3Codes<W>::KS, NT = E4m3Codes<W>::NT;
+  half8_t q[KS][2];    // row c, dims 32u + 16h + 8x ..
   f32x16_t o[NT];
-  float base, thr, sum;              // of the row; `sum` over the lane's own tokens
-  int lim;                           // the row's last visible position within the item
-  int first_lim, last_lim;           // over the wave's rows (wave-uniform)
+  f32x16_t start;      // -base, sixteen times: the scores' start (0 when they are scaled afterwards)
+  float base, thr, sum;  // of the row; `sum` over the lane's own tokens
+  float after;         // factor of the scores once q has entered unscaled, or 0
+  int lim;             // the row's last visible position within the item
+  int first_lim, last_lim;  // over the wave's rows (wave-uniform)
 
-  // Tokens [16 * page, 16 * page + 32) from the two blocks at `slot`.
-  __device__ __forceinline__ void pair(const char* slot, uint32_t sa, uint32_t sb, int page, int lane) {
-    constexpr int BLOCK = E4m3Cfg<W>::BLOCK;
-    const int c = lane & 31, h = lane >> 5;
-    const float ks = __uint_as_float((c & 16 ? sb : sa) << 16);
-    const char* kp = slot + (c >> 4) * BLOCK + h * 256 + (c & 15) * 16;
-    f32x16_t s;
+  __device__ __forceinline__ void set_start() {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = -base;
+    for (int r = 0; r < 16; ++r) start[r] = after != 0.0f ? 0.0f : -base;
+  }
+
+  // Tokens [16 * page, 16 * page + 32).
+  __device__ __forceinline__ void pair(const E4m3Codes<W>& x, int page, int lane) {
+    const int c = lane & 31, h = lane >> 5;
+    const float ks = __uint_as_float((c & 16 ? x.sb : x.sa) << 16);
+    f32x16_t s = start;
 #pragma unroll
     for (int u = 0; u < KS; ++u) {
-      const u32x4_t k = *reinterpret_cast<const u32x4_t*>(kp + u * 512);
-      s = MFMA32x32x16(e4m3x8(k[0], k[1], ks), q[u][0], s);
-      s = MFMA32x32x16(e4m3x8(k[2], k[3], ks), q[u][1], s);
+      s = MFMA32x32x16(e4m3x8(x.k[u][0], x.k[u][1], ks), q[u][0], s);
+      s = MFMA32x32x16(e4m3x8(x.k[u][2], x.k[u][3], ks), q[u][1], s);
+    }
+    if (after != 0.0f) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], after, -base);
     }
     if (page * 16 + 31 > first_lim) {  // (wave-uniform: positions that some row does not see)
       const int p0 = page * 16 + 4 * h;
@@ -168,6 +215,7 @@ struct E4m3Rows {
       sum *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
+      set_start();
     }
     half8_t p[2];
     const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
@@ -181,28 +229,9 @@ struct E4m3Rows {
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const float vs = __uint_as_float((b ? sb : sa) & 0xffff0000u);
-      const char* vp = slot + b * BLOCK + 16 * W + (h * 16 + (c & 15)) * 16;
-      uint32_t x[NT], y[NT];  // tokens 4h .. and 8 + 4h .. of dims 32i + c
-      if constexpr (W == 64) {
-        const u32x2_t a = *reinterpret_cast<const u32x2_t*>(vp + (c >> 4) * 8);
-        const u32x2_t d = *reinterpret_cast<const u32x2_t*>(vp + (c >> 4) * 8 + 512);
-        x[0] = a[0]; x[1] = a[1]; y[0] = d[0]; y[1] = d[1];
-      } else {
-        const char* vq = vp + (c >> 4) * (8 * W);
+      const float vs = __uint_as_float((b ? x.sb : x.sa) & 0xffff0000u);
 #pragma unroll
-        for (int k = 0; k < NT / 4; ++k) {
-          const u32x4_t a = *reinterpret_cast<const u32x4_t*>(vq + k * 1024);
-          const u32x4_t d = *reinterpret_cast<const u32x4_t*>(vq + k * 1024 + 512);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[4 * k + i] = a[i];
-            y[4 * k + i] = d[i];
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) o[i] = MFMA32x32x16(e4m3x8(x[i], y[i], vs), p[b], o[i]);
+      for (int i = 0; i < NT; ++i) o[i] = MFMA32x32x16(e4m3x8(x.v[b][0][i], x.v[b][1][i], vs), p[b], o[i]);
     }
   }
 };
@@ -222,6 +251,7 @@ __device__ __forceinline__ E4m3Item load_item(const E4m3Item* items, int i) {
   t.merge = w[9];
   t.rw = w[10];
   t.once = w[11];
+  t.next = w[12];
   return t;
 }
 
@@ -230,6 +260,107 @@ __device__ __forceinline__ E4m3Item load_item(const E4m3Item* items, int i) {
 template <int W>
 __device__ __forceinline__ int staged(int r, int c) {
   return r * W * 4 + ((c ^ (r & (W / 4 - 1))) << 4);
+}
+
+// threadIdx.x, computed anew wherever this is called: without it the compiler
+// moves every address of the item's end in front of the item loop and spills.
+__device__ __forceinline__ int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// Adds the pieces of J chunks of 4 dims a thread, K pieces in flight.
+template <int W, int J, int K>
+__device__ __forceinline__ void add_parts(const E4m3Attn& p, const E4m3Shared<W>& sh, const E4m3Merge& m,
+                                          __amdgpu_buffer_rsrc_t rs_o, __amdgpu_buffer_rsrc_t rs_ml,
+                                          const float2* ml, bool fits, int t) {
+  const int rows = m.rows, n = m.n_parts, chunks = rows * (W / 4);
+#pragma unroll 1
+  for (int i0 = t; i0 < chunks; i0 += 256 * J) {
+    float4_t acc[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] = float4_t{0, 0, 0, 0};
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += K) {
+      float4_t o[J][K];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int idx = min(i0 + 256 * j, chunks - 1), r = idx / (W / 4), d4 = idx % (W / 4);
+#pragma unroll
+        for (int e = 0; e < K; ++e)
+          o[j][e] = coh_load4(rs_o, (uint32_t)((((size_t)(m.first_part + min(k0 + e, n - 1)) * kE4m3Rows + r) * W + 4 * d4) * 4));
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int r = min(i0 + 256 * j, chunks - 1) / (W / 4);
+#pragma unroll
+        for (int e = 0; e < K; ++e) {
+          float w = 0.0f;
+          if (fits) {
+            w = ml[min(k0 + e, n - 1) * rows + r].x;
+          } else {
+            const float x =
+                coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + min(k0 + e, n - 1)) * kE4m3Rows + r) * 8)).x;
+            w = x == -INFINITY ? 0.0f : pow2i(x - sh.base[r]);
+          }
+          if (k0 + e < n) acc[j] += o[j][e] * w;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int idx = i0 + 256 * j, r = idx / (W / 4), d4 = idx % (W / 4);
+      if (idx < chunks && 4 * d4 < p.dims) {
+        const float sum = sh.sum[r];
+        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
+                   sum > 0.0f || sum != sum ? div4(acc[j], sum) : float4_t{0, 0, 0, 0});
+      }
+    }
+  }
+}
+
+// The states of a split tile's pieces become its output: the pieces' maxima
+// and sums are read at once and turned into weights in LDS, then every thread
+// adds its chunks. The sums are in the pieces' order.
+template <int W>
+__device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh, const E4m3Item& it,
+                                            const E4m3Merge& m) {
+  const auto rs_o = make_rsrc(p.part_o, 0x7fffffff);
+  const auto rs_ml = make_rsrc(p.part_ml, 0x7fffffff);
+  const int t = thread_here(), rows = m.rows, n = m.n_parts;
+  float2* const ml = reinterpret_cast<float2*>(sh.ring);  // [n][rows]: (base, sum), then (weight, -)
+  const bool fits = (size_t)n * rows * sizeof(float2) <= sizeof(sh.ring);  // else they are read where they are used
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  auto state = [&](int k, int r) __attribute__((always_inline)) {
+    return coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + k) * kE4m3Rows + r) * 8));
+  };
+  if (fits) {
+#pragma unroll 4
+    for (int i = t; i < n * rows; i += 256) ml[i] = state(i / rows, i % rows);
+    __syncthreads();
+  }
+  if (t < rows) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) top = fmaxf(top, fits ? ml[k * rows + t].x : state(k, t).x);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float2 v = fits ? ml[k * rows + t] : state(k, t);
+      const float w = v.x == -INFINITY ? 0.0f : pow2i(v.x - top);
+      sum += w * v.y;
+      if (fits) ml[k * rows + t].x = w;
+    }
+    sh.base[t] = top;
+    sh.sum[t] = sum;
+  }
+  __syncthreads();
+  // (16 loads in flight either way)
+  if (rows * (W / 4) <= 256)
+    add_parts<W, 1, 16>(p, sh, m, rs_o, rs_ml, ml, fits, t);
+  else
+    add_parts<W, 4, 4>(p, sh, m, rs_o, rs_ml, ml, fits, t);
+  if (t == 0) __hip_atomic_store(p.counters + it.merge, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 template <int W, int RW>
@@ -247,8 +378,11 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
   const int turns = (ntiles + KS - 1) / KS;
 
   // ---- the item's block numbers and rows
-  for (int j = threadIdx.x; j < npages; j += 256)
-    sh.ids[j] = p.tables[it.table_off + it.page_begin + j] * p.kv_heads + it.kv_head;
+  // (to a whole number of tiles: pages past the range repeat the last one,
+  // whose positions there no row sees)
+  const int padded = (npages + 7) & ~7;
+  for (int j = threadIdx.x; j < padded; j += 256)
+    sh.ids[j] = p.tables[it.table_off + it.page_begin + min(j, npages - 1)] * p.kv_heads + it.kv_head;
   if ((int)threadIdx.x < it.rows) {
     const int r = it.row0 + threadIdx.x, query = r / p.group;
     sh.out_at[threadIdx.x] = (long)(it.q_row + query) * p.out_stride +
@@ -257,27 +391,36 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
   __syncthreads();
 
   char* const ring = sh.ring + ks * NB * TP * C::BLOCK;
-  // Tile `turn * KS + ks` of the item into its slot; pages past the range
-  // repeat the last one (no row sees their positions).
+  // Tile `turn * KS + ks` of the item into its slot (a group past the item's
+  // last tile copies that one again).
   auto fetch = [&](int turn) __attribute__((always_inline)) {
     char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
-    const int j0 = (turn * KS + ks) * TP + wr * MINE;
+    const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
+    int n[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) n[i] = sh.ids[j0 + i];
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      const int n = __builtin_amdgcn_readfirstlane(sh.ids[min(j0 + i, npages - 1)]);
+      const int block = __builtin_amdgcn_readfirstlane(n[i]);
       if (it.once)
-        fetch_block<W, kPageLoadPolicy>(slot + i * C::BLOCK, p.blocks, n, lane);
+        fetch_block<W, kPageLoadPolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
       else
-        fetch_block<W, kPageReusePolicy>(slot + i * C::BLOCK, p.blocks, n, lane);
+        fetch_block<W, kPageReusePolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
     }
   };
+  constexpr int AHEAD = RW == 1 ? NB : NB - 1;  // tiles copied before the first is used
 #pragma unroll
-  for (int k = 0; k < NB - 1; ++k)
+  for (int k = 0; k < AHEAD; ++k)
     if (k < turns) fetch(k);
-  for (int j = threadIdx.x; j < npages; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
+  for (int j = threadIdx.x; j < padded; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
 
   E4m3Rows<W> x;
   {
+    // f16 rows enter the products as they are and the scores are scaled
+    // afterwards; scaled first, their second rounding doubles the error of an
+    // f16 output. (fp32 and bf16 rows are scaled and rounded to f16 once.)
+    x.after = p.row_type == TGE_ROWS_F16 ? p.scale_log2 : 0.0f;
+    const float factor = p.row_type == TGE_ROWS_F16 ? 1.0f : p.scale_log2;
     const int r = wr * 32 + c;
     const bool live = r < it.rows;
     const int g = it.row0 + (live ? r : 0), query = g / p.group;
@@ -292,12 +435,13 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int d = 32 * u + 16 * h + 8 * e;
-        x.q[u][e] = live && d < p.dims ? load_q8(p.q, at + d, p.row_type, p.scale_log2) : half8_t{};
+        x.q[u][e] = live && d < p.dims ? load_q8(p.q, at + d, p.row_type, factor) : half8_t{};
       }
     }
     x.base = 0.0f;
     x.thr = -INFINITY;
     x.sum = 0.0f;
+    x.set_start();
 #pragma unroll
     for (int i = 0; i < E4m3Rows<W>::NT; ++i)
 #pragma unroll
@@ -306,31 +450,37 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
   __syncthreads();  // scales are in LDS
 
   for (int turn = 0; turn < turns; ++turn) {
+    char* const slot = ring + (turn % NB) * TP * C::BLOCK;
+    const int j0 = (turn * KS + ks) * TP;
+    const int page = it.page_begin + j0;
     if constexpr (RW == 1) {
-      if (turn + NB - 1 < turns) {
-        fetch(turn + NB - 1);
+      // The wave's own ring: once a tile's codes are in registers its slot
+      // takes the tile NB turns on, so NB tiles are in flight while one is
+      // worked on.
+      if (turn + 1 < turns)
         wait_vmcnt<(NB - 1) * LOADS>();
-      } else {
+      else
         wait_vmcnt<0>();
-      }
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      const int j = min(j0, padded - TP);
+      E4m3Codes<W> codes;
+      codes.read(slot, sh.scales + j, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (turn + NB < turns) fetch(turn + NB);
+      if (j0 < npages && page * 16 <= x.last_lim) x.pair(codes, page, lane);
     } else {
       wait_vmcnt_pages<NB - 2, LOADS>(min(NB - 2, turns - 1 - turn));
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (turn + NB - 1 < turns) fetch(turn + NB - 1);
-    }
-    const char* const slot = ring + (turn % NB) * TP * C::BLOCK;
-    const int j0 = (turn * KS + ks) * TP;
 #pragma unroll
-    for (int b = 0; b < TP; b += 2) {
-      const int page = it.page_begin + j0 + b;
-      if (j0 + b < npages && page * 16 <= x.last_lim) {
-        const uint32_t sa = __builtin_amdgcn_readfirstlane(sh.scales[j0 + b]);
-        const uint32_t sb = __builtin_amdgcn_readfirstlane(sh.scales[min(j0 + b + 1, npages - 1)]);
-        x.pair(slot + b * C::BLOCK, sa, sb, page, lane);
+      for (int b = 0; b < TP; b += 2) {
+        if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
+          E4m3Codes<W> codes;
+          codes.read(slot + b * C::BLOCK, sh.scales + j0 + b, lane);
+          x.pair(codes, page + b, lane);
+        }
       }
     }
-    if constexpr (RW == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 
   // ---- the groups' states become one: common bases, sums, accumulators
@@ -365,25 +515,34 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
       *reinterpret_cast<float4_t*>(stage + staged<W>(c, 8 * i + 2 * e + h)) =
           float4_t{x.o[i][4 * e], x.o[i][4 * e + 1], x.o[i][4 * e + 2], x.o[i][4 * e + 3]} * f;
   __syncthreads();
+}
+
+// The staged accumulators of the item's waves become output rows or, for a
+// piece of a split tile, a partial state; the last piece of a tile to arrive
+// merges them all.
+template <int W>
+__device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh, const E4m3Item& it) {
+  __syncthreads();
+  const int rw = it.rw, copies = 4 / rw;
   const auto rs_o = make_rsrc(p.part_o, 0x7fffffff);
   const auto rs_ml = make_rsrc(p.part_ml, 0x7fffffff);
-  for (int idx = threadIdx.x; idx < it.rows * (W / 4); idx += 256) {
+#pragma unroll 2
+  for (int idx = thread_here(); idx < it.rows * (W / 4); idx += 256) {
     const int r = idx / (W / 4), d4 = idx % (W / 4);
-    float4_t acc = {0, 0, 0, 0};
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-      acc += *reinterpret_cast<const float4_t*>(sh.ring + (k * RW + (r >> 5)) * 32 * W * 4 + staged<W>(r & 31, d4));
+    const char* from = sh.ring + (r >> 5) * 32 * W * 4 + staged<W>(r & 31, d4);
+    float4_t acc = *reinterpret_cast<const float4_t*>(from);
+    for (int k = 1; k < copies; ++k) acc += *reinterpret_cast<const float4_t*>(from + k * rw * 32 * W * 4);
     if (it.part < 0) {
       const float sum = sh.sum[r];
       if (4 * d4 < p.dims)
-        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type, sum > 0.0f || sum != sum ? div4(acc, sum) : float4_t{0, 0, 0, 0});
+        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
+                   sum > 0.0f || sum != sum ? div4(acc, sum) : float4_t{0, 0, 0, 0});
     } else {
       coh_store4(rs_o, (uint32_t)((((size_t)it.part * kE4m3Rows + r) * W + 4 * d4) * 4), acc);
       if (d4 == 0) coh_store2(rs_ml, (uint32_t)(((size_t)it.part * kE4m3Rows + r) * 8), sh.base[r], sh.sum[r]);
     }
   }
   if (it.part >= 0) {
-    // The last piece of the tile to arrive merges them all, in their order.
     const E4m3Merge m = p.merges[it.merge];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     wait_vmcnt<0>();
@@ -392,36 +551,7 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
       sh.flag = __hip_atomic_fetch_add(p.counters + it.merge, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                 m.n_parts - 1;
     __syncthreads();
-    if (sh.flag) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-      if ((int)threadIdx.x < m.rows) {
-        float mm = -INFINITY, sum = 0.0f;
-        for (int k = 0; k < m.n_parts; ++k) {
-          const float2 v = coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + k) * kE4m3Rows + threadIdx.x) * 8));
-          if (v.x == -INFINITY) continue;
-          const float t = fmaxf(mm, v.x);
-          sum = (mm == -INFINITY ? 0.0f : sum * pow2i(mm - t)) + v.y * pow2i(v.x - t);
-          mm = t;
-        }
-        sh.base[threadIdx.x] = mm;
-        sh.sum[threadIdx.x] = sum;
-      }
-      __syncthreads();
-      for (int idx = threadIdx.x; idx < m.rows * (W / 4); idx += 256) {
-        const int r = idx / (W / 4), d4 = idx % (W / 4);
-        const float mm = sh.base[r], sum = sh.sum[r];
-        float4_t acc = {0, 0, 0, 0};
-        for (int k = 0; k < m.n_parts; ++k) {
-          const size_t at = (size_t)(m.first_part + k) * kE4m3Rows + r;
-          const float2 v = coh_load2(rs_ml, (uint32_t)(at * 8));
-          const float4_t o = coh_load4(rs_o, (uint32_t)((at * W + 4 * d4) * 4));
-          if (v.x != -INFINITY) acc += o * pow2i(v.x - mm);
-        }
-        if (4 * d4 < p.dims)
-          store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type, sum > 0.0f || sum != sum ? div4(acc, sum) : float4_t{0, 0, 0, 0});
-      }
-      if (threadIdx.x == 0) __hip_atomic_store(p.counters + it.merge, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if (sh.flag) merge_parts<W>(p, sh, it, m);
   }
   __syncthreads();  // the shared state is free for the next item
 }
@@ -430,15 +560,16 @@ template <int W>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(E4m3Cfg<W>::PER_CU, E4m3Cfg<W>::PER_CU)))
 void attention_e4m3_kernel(E4m3Attn p) {
   __shared__ E4m3Shared<W> sh;
-  const int first = p.wg_first[blockIdx.x], last = p.wg_first[blockIdx.x + 1];
-  for (int i = first; i < last; ++i) {
+  for (int i = blockIdx.x; i >= 0;) {
     const E4m3Item it = load_item(p.items, i);
+    i = it.next;
     if (it.rw == 1)
       run_item<W, 1>(p, sh, it);
     else if (it.rw == 2)
       run_item<W, 2>(p, sh, it);
     else
       run_item<W, 4>(p, sh, it);
+    finish_item<W>(p, sh, it);
   }
 }
 

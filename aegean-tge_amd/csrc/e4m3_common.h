@@ -80,7 +80,8 @@ struct E4m3Item {
   int merge;       // merge record of a split tile, or -1
   int rw;          // row-waves: 1, 2 or 4 waves of 32 rows; 4 / rw waves share the pages
   int once;        // 1: no other item reads these blocks (cache policy of the loads)
-  int pad[4];
+  int next;        // the workgroup's next item, or -1
+  int pad[3];
 };
 static_assert(sizeof(E4m3Item) == 16 * sizeof(int), "E4m3Item is read as 16 ints");
 

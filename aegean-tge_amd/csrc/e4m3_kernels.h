@@ -40,8 +40,7 @@ struct E4m3Append {
 struct E4m3Attn {
   const char* blocks;
   const uint32_t* scales;
-  const E4m3Item* items;
-  const int* wg_first;  // [groups + 1]
+  const E4m3Item* items;  // workgroup i starts with item i
   const int* tables;
   const E4m3Merge* merges;
   int* counters;  // arrivals of each merge record, zero between launches

@@ -181,7 +181,7 @@ struct StepPlan {
 struct E4m3Plan {
   tge::plan::E4m3Lists lists;
   bool built = false;
-  size_t off_tiles = 0, off_items = 0, off_first = 0, off_merges = 0, off_counters = 0;  // in the batch image
+  size_t off_tiles = 0, off_items = 0, off_merges = 0, off_counters = 0;  // in the batch image
   tge::plan::Scratch part_o, part_ml;
   ~E4m3Plan() {
     part_o.release(g_mem);
@@ -527,7 +527,7 @@ int finish_step_plan(tge_batch* b, hipStream_t st) {
 }
 
 // The e4m3 part of tge_batch_plan: one upload holds
-// [ tables | rows | append tiles | items | wg_first | merges | counters ].
+// [ tables | rows | append tiles | items | merges | counters ].
 int plan_e4m3(tge_batch* b, hipStream_t hs) {
   const tge::plan::Step& st = b->step;
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -537,15 +537,14 @@ int plan_e4m3(tge_batch* b, hipStream_t hs) {
                 "batch_plan: the stream is capturing (the plan is uploaded from host memory, which a "
                 "graph would replay stale; plan first, then capture the calls)");
   E4m3Plan& e = b->e4;
-  tge::plan::build_e4m3(st, device_cus() * tge::e4m3_groups_per_cu(st.block_dims), e.lists);
+  tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
   const auto& L = e.lists;
   if ((size_t)L.parts * tge::kE4m3Rows * st.block_dims * sizeof(float) > 0x7fffffffu)
     return fail(TGE_ERR_CAPACITY, "batch_plan: the step's partial states exceed 2 GiB");
   const size_t o_rows = align_up(st.tables.size() * sizeof(int));
   e.off_tiles = align_up(o_rows + st.rows.size() * sizeof(tge::RowRec));
   e.off_items = align_up(e.off_tiles + L.tiles.size() * sizeof(tge::E4m3Tile));
-  e.off_first = align_up(e.off_items + L.items.size() * sizeof(tge::E4m3Item));
-  e.off_merges = align_up(e.off_first + L.wg_first.size() * sizeof(int));
+  e.off_merges = align_up(e.off_items + L.items.size() * sizeof(tge::E4m3Item));
   e.off_counters = align_up(e.off_merges + L.merges.size() * sizeof(tge::E4m3Merge));
   const size_t total = e.off_counters + L.merges.size() * sizeof(int);
   int s = b->image.upload(g_mem, total, hs, [&](char* h) {
@@ -556,7 +555,6 @@ int plan_e4m3(tge_batch* b, hipStream_t hs) {
     put(o_rows, st.rows);
     put(e.off_tiles, L.tiles);
     put(e.off_items, L.items);
-    put(e.off_first, L.wg_first);
     put(e.off_merges, L.merges);
     if (!L.merges.empty()) std::memset(h + e.off_counters, 0, L.merges.size() * sizeof(int));
   });
@@ -960,7 +958,6 @@ int attention_params_e4m3(const tge_batch* b, const tge_kv_pool* p, int layer, c
   x.blocks = static_cast<const char*>(view.k);
   x.scales = static_cast<const uint32_t*>(view.k_scales);
   x.items = reinterpret_cast<const tge::E4m3Item*>(b->image.dev + e.off_items);
-  x.wg_first = reinterpret_cast<const int*>(b->image.dev + e.off_first);
   x.tables = reinterpret_cast<const int*>(b->image.dev + b->off_tables);
   x.merges = reinterpret_cast<const tge::E4m3Merge*>(b->image.dev + e.off_merges);
   x.counters = reinterpret_cast<int*>(b->image.dev + e.off_counters);

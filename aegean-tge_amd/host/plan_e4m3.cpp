@@ -2,28 +2,173 @@
 #include "plan_e4m3.hpp"
 
 #include <algorithm>
+#include <cstdlib>
+#include <utility>
 
 namespace tge::plan {
 
 namespace {
 
-// Pages a piece of a split tile has at least; a workgroup's start and the
-// merge cost about as much as this many pages.
-constexpr int kMinPages = 32;
-constexpr int kStartPages = 12;
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
+// Rows of one (session, KV head) that meet the same pages, and what they cost
+// a workgroup.
 struct Tile {
   int session, kv_head, row0, rows, rw, pages;
 };
 
+// A piece of a tile: pages [begin, end), the piece `index` of `of`.
+struct Piece {
+  int tile, begin, end, index, of;
+};
+
+using Group = std::vector<Piece>;
+
+// Costs in microseconds of a workgroup while every slot is busy, fitted to
+// launches of 0.5 to 280 GFLOP with every tile size and way to cut.
+struct Costs {
+  double page;    // a page
+  double start;   // an item's start and end
+  double merge;   // a tile that is cut: its merge
+  double solo;    // cost of an item, relative, where most slots are idle
+  double spread;  // cost of a page, relative, in shares: neighbours are at different pages and share the L2 less
+  int grain;      // pages that the waves share out at a time
+  int least;      // pages of a piece
+
+  double time(double total, double longest, int slots, bool cut) const {
+    return std::max(total / slots + 0.3 * longest, solo * longest) + (cut ? merge : 0.0);
+  }
+};
+
+// A decode page is bound by HBM (4 KiB at 512 workgroups' shares of 5.6 TB/s),
+// a prompt page by the matrix cores and the exponentials; waves that share
+// their pages (a larger rw) pay less for the copies.
+Costs costs_of(int rw, bool prompt, int width) {
+  const double w = width / 128.0;
+  if (!prompt) return Costs{0.37 * w, 4.5, 4.0, 0.25, 1.0, 8, 32};
+  const double page = rw == 1 ? 0.155 : rw == 2 ? 0.32 : 0.45;
+  return Costs{page * w, 5.0, 6.0 + 2.0 * rw, 0.75, 1.35, rw == 1 ? 8 : 4, 32};
+}
+
+// Each tile in equal pieces, a piece a group: the shortest pieces that fit.
+std::vector<Group> one_each(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
+  int most = 0;
+  for (const Tile& t : tiles) most = std::max(most, t.pages);
+  int lo = c.least, hi = std::max(most, c.least);
+  auto count = [&](int p) {
+    long long n = 0;
+    for (const Tile& t : tiles) n += ceil_div(t.pages, p);
+    return n;
+  };
+  hi = std::min(hi, kE4m3ItemPages);
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (count(mid) <= slots)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  std::vector<Group> groups;
+  double longest = 0.0, total = 0.0;
+  bool cut = false;
+  for (std::size_t i = 0; i < tiles.size(); ++i) {
+    const int n = ceil_div(tiles[i].pages, lo), len = ceil_div(ceil_div(tiles[i].pages, n), c.grain) * c.grain;
+    const int of = ceil_div(tiles[i].pages, len);
+    for (int k = 0; k < of; ++k)
+      groups.push_back({Piece{(int)i, k * len, std::min((k + 1) * len, tiles[i].pages), k, of}});
+    longest = std::max(longest, std::min(len, tiles[i].pages) * c.page + c.start);
+    total += tiles[i].pages * c.page + of * c.start;
+    cut = cut || of > 1;
+  }
+  *time = c.time(total, longest, slots, cut);
+  return groups;
+}
+
+// The tiles end to end, cut into shares, a share a group. Workgroups that land
+// on a compute unit after others get less of it (equal shares of a decode
+// launch end after 65 and 80 us, two workgroups a unit), so the share of the
+// k-th of `per_cu` is smaller by `kLater` for each one before it.
+constexpr double kLater = 0.18;
+std::vector<Group> shares(const std::vector<Tile>& tiles, int slots, int per_cu, const Costs& c, double* time) {
+  double total = 0.0;
+  for (const Tile& t : tiles) total += t.pages * c.page + c.start;
+  const int least = std::min(c.least, 2 * c.grain), cus = std::max(1, slots / per_cu);
+  const double middle = 1.0 - kLater * (per_cu - 1) / 2;
+  double share = std::max(total / slots + 0.5 * c.start, c.least * c.page + c.start);
+  std::vector<Group> groups;
+  bool cut = false;
+  for (;; share *= 1.01) {  // (until the shares are no more than the slots)
+    groups.clear();
+    cut = false;
+    double left = 0.0;
+    for (std::size_t i = 0; i < tiles.size(); ++i) {
+      const int pages = tiles[i].pages;
+      std::vector<std::pair<int, int>> at;  // (end page, group) of each piece
+      for (int begin = 0; begin < pages;) {
+        if (left < c.start + least * c.page || groups.empty()) {
+          const int later = std::min((int)groups.size() / cus, per_cu - 1);
+          left = share * (1.0 - kLater * later) / middle;
+          groups.emplace_back();
+        }
+        int n = std::min(pages - begin, std::max(least, (int)((left - c.start) / c.page) / c.grain * c.grain));
+        if (pages - begin - n < least) n = pages - begin;  // (no slivers)
+        n = std::min(n, kE4m3ItemPages);
+        begin += n;
+        left -= n * c.page + c.start;
+        at.emplace_back(begin, (int)groups.size() - 1);
+      }
+      cut = cut || at.size() > 1;
+      for (std::size_t k = 0; k < at.size(); ++k)
+        groups[(std::size_t)at[k].second].push_back(
+            Piece{(int)i, k ? at[k - 1].first : 0, at[k].first, (int)k, (int)at.size()});
+    }
+    if ((int)groups.size() <= slots) break;
+  }
+  *time = c.spread * share + 0.3 * c.start + (cut ? c.merge : 0.0);
+  return groups;
+}
+
+// Whole tiles, the longest first (more tiles than slots: the device takes the
+// next one as a slot falls free).
+std::vector<Group> whole(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
+  std::vector<std::size_t> order(tiles.size());
+  for (std::size_t i = 0; i < order.size(); ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(),
+                   [&](std::size_t a, std::size_t b) { return tiles[a].pages > tiles[b].pages; });
+  std::vector<Group> groups(tiles.size());
+  double longest = 0.0, total = 0.0;
+  for (std::size_t k = 0; k < order.size(); ++k) {
+    const int pages = tiles[order[k]].pages, of = ceil_div(pages, kE4m3ItemPages);
+    for (int p = 0; p < of; ++p)
+      groups[k].push_back(Piece{(int)order[k], p * kE4m3ItemPages, std::min((p + 1) * kE4m3ItemPages, pages), p, of});
+    const double t = pages * c.page + of * c.start;
+    longest = std::max(longest, t);
+    total += t;
+  }
+  *time = c.time(total, longest, slots, false);
+  return groups;
+}
+
+// Workgroup b runs on XCD b mod 8, each with an L2 of its own: neighbours in
+// the list, which read the same pages, go to one XCD.
+std::vector<Group> by_xcd(std::vector<Group> groups) {
+  const std::size_t n = groups.size(), x = 8;
+  std::vector<Group> out;
+  out.reserve(n);
+  for (std::size_t i = 0; i < n; ++i) {
+    // chunk i % 8 starts after the chunks before it (the first n % 8 hold one more)
+    const std::size_t chunk = i % x, per = n / x, more = n % x;
+    out.push_back(std::move(groups[chunk * per + std::min(chunk, more) + i / x]));
+  }
+  return out;
+}
+
 }  // namespace
 
-void build_e4m3(const Step& s, int slots, E4m3Lists& out) {
+void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
+  const int slots = cus * per_cu;
   out.tiles.clear();
   out.items.clear();
-  out.wg_first.clear();
   out.merges.clear();
   out.groups = out.parts = 0;
   out.page_twice = false;
@@ -44,101 +189,117 @@ void build_e4m3(const Step& s, int slots, E4m3Lists& out) {
     seen[(std::size_t)t.page] = 1;
   }
 
-  // ---- attention: tiles of rows. Sessions of up to 64 rows a KV head are one
-  // tile, whose blocks nothing else reads; longer ones are cut into the
-  // largest tiles that still fill the device, since a larger tile reads its
-  // pages less often.
+  // ---- attention. Sessions of up to 64 rows a KV head are one tile each,
+  // whose pages nothing else reads.
   const int g = s.group;
-  long long prompt_rows = 0;
-  for (const SessionRec& r : s.sessions)
-    if (r.n_new * g > 64) prompt_rows += r.n_new * g;
-  int prw = 4;
-  while (prw > 1 && (prompt_rows * s.kv_heads) / (32 * prw) < slots) prw /= 2;
-  std::vector<Tile> once, again;
+  std::vector<Tile> decode;
+  bool prompts = false;
   for (std::size_t i = 0; i < s.sessions.size(); ++i) {
     const SessionRec& r = s.sessions[i];
     const int rows = r.n_new * g;
-    if (rows <= 64) {
-      for (int h = 0; h < s.kv_heads; ++h)
-        once.push_back(Tile{(int)i, h, 0, rows, rows <= 32 ? 1 : 2, ceil_div(r.ctx + r.n_new, 16)});
+    if (rows > 64) {
+      prompts = true;
       continue;
     }
-    for (int row0 = 0; row0 < rows; row0 += 32 * prw) {
-      const int n = std::min(32 * prw, rows - row0);
-      for (int h = 0; h < s.kv_heads; ++h)
-        again.push_back(Tile{(int)i, h, row0, n, prw, ceil_div(r.ctx + (row0 + n - 1) / g + 1, 16)});
-    }
+    for (int h = 0; h < s.kv_heads; ++h)
+      decode.push_back(Tile{(int)i, h, 0, rows, rows <= 32 ? 1 : 2, ceil_div(r.ctx + r.n_new, 16)});
   }
-  auto emit = [&](const Tile& t, int begin, int end, int part, int merge, int once_flag) {
-    const SessionRec& r = s.sessions[(std::size_t)t.session];
-    out.items.push_back(E4m3Item{t.kv_head, begin, end, part, t.row0, t.rows, r.ctx, r.q_row, r.table_off, merge,
-                                 t.rw, once_flag, {}});
-  };
-  auto merge_of = [&](const Tile& t, int n) {
-    const SessionRec& r = s.sessions[(std::size_t)t.session];
-    out.merges.push_back(E4m3Merge{out.parts, n, t.rows, t.row0, t.kv_head, r.q_row, {}});
-    out.parts += n;
-    return (int)out.merges.size() - 1;
+  auto prompt_tiles = [&](int rw) {
+    std::vector<Tile> t;
+    for (std::size_t i = 0; i < s.sessions.size(); ++i) {
+      const SessionRec& r = s.sessions[i];
+      const int rows = r.n_new * g;
+      for (int h = 0; rows > 64 && h < s.kv_heads; ++h)
+        for (int row0 = 0; row0 < rows; row0 += 32 * rw) {
+          const int n = std::min(32 * rw, rows - row0);
+          t.push_back(Tile{(int)i, h, row0, n, rw, ceil_div(r.ctx + (row0 + n - 1) / g + 1, 16)});
+        }
+    }
+    return t;
   };
 
-  // Tiles read once: laid end to end and cut into equal shares.
-  long long cost = 0;
-  for (const Tile& t : once) cost += t.pages + kStartPages;
-  const long long share = std::max<long long>(kMinPages + kStartPages, (cost + slots - 1) / slots);
-  long long left = 0;  // of the current workgroup's share
-  for (const Tile& t : once) {
-    // the pieces of this tile: end page, and whether a workgroup starts with the piece
-    std::vector<std::pair<int, bool>> cuts;
-    for (int at = 0; at < t.pages;) {
-      const bool fresh = left < kStartPages + 8;
-      if (fresh) left = share;
-      int n = (int)std::min<long long>(t.pages - at, left - kStartPages);
-      if (n < t.pages - at) n = n / 8 * 8;
-      if (t.pages - at - n < 8) n = t.pages - at;  // no slivers
-      n = std::min(n, kE4m3ItemPages);
-      left -= n + kStartPages;
-      at += n;
-      cuts.emplace_back(at, fresh);
-    }
-    const int n = (int)cuts.size(), first = out.parts;
-    const int merge = n > 1 ? merge_of(t, n) : -1;
-    int at = 0;
-    for (int i = 0; i < n; ++i) {
-      if (cuts[(std::size_t)i].second) out.wg_first.push_back((int)out.items.size());
-      emit(t, at, cuts[(std::size_t)i].first, n > 1 ? first + i : -1, merge, 1);
-      at = cuts[(std::size_t)i].first;
-    }
-  }
-
-  // Prompt tiles: one piece a workgroup, the longest first; pieces of a tile
-  // are of equal length, short enough to fill the device.
-  if (!again.empty()) {
-    long long pages = 0;
-    for (const Tile& t : again) pages += t.pages;
-    const int most = (int)std::min<long long>(
-        kE4m3ItemPages, std::max<long long>(kMinPages, (pages + slots - 1) / slots));
-    std::vector<int> cut(again.size());
-    const bool fill = (int)again.size() < slots;  // fewer tiles than workgroups
-    for (std::size_t i = 0; i < again.size(); ++i)
-      cut[i] = ceil_div(again[i].pages, fill ? most : kE4m3ItemPages);
-    std::vector<std::size_t> order(again.size());
-    for (std::size_t i = 0; i < order.size(); ++i) order[i] = i;
-    std::stable_sort(order.begin(), order.end(), [&](std::size_t a, std::size_t b) {
-      return ceil_div(again[a].pages, cut[a]) > ceil_div(again[b].pages, cut[b]);
-    });
-    for (std::size_t i : order) {
-      const Tile& t = again[i];
-      const int n = cut[i], first = out.parts;
-      const int merge = n > 1 ? merge_of(t, n) : -1;
-      for (int k = 0; k < n; ++k) {
-        out.wg_first.push_back((int)out.items.size());
-        emit(t, (int)((long long)t.pages * k / n), (int)((long long)t.pages * (k + 1) / n), n > 1 ? first + k : -1,
-             merge, 0);
+  std::vector<std::vector<E4m3Item>> all;
+  auto add = [&](const std::vector<Tile>& tiles, const std::vector<Group>& groups, bool once) {
+    // pieces of a cut tile own consecutive partial slots
+    std::vector<int> merge(tiles.size(), -1);
+    for (const Group& gr : groups) {
+      all.emplace_back();
+      for (const Piece& p : gr) {
+        const Tile& t = tiles[(std::size_t)p.tile];
+        const SessionRec& r = s.sessions[(std::size_t)t.session];
+        int& m = merge[(std::size_t)p.tile];
+        if (p.of > 1 && m < 0) {
+          m = (int)out.merges.size();
+          out.merges.push_back(E4m3Merge{out.parts, p.of, t.rows, t.row0, t.kv_head, r.q_row, {}});
+          out.parts += p.of;
+        }
+        const int part = p.of > 1 ? out.merges[(std::size_t)m].first_part + p.index : -1;
+        all.back().push_back(E4m3Item{t.kv_head, p.begin, p.end, part, t.row0, t.rows, r.ctx, r.q_row, r.table_off, m,
+                                      t.rw, once ? 1 : 0, -1, {}});
       }
     }
+  };
+
+  double time = 0.0;
+  auto plan_decode = [&](int n, double* t) {
+    const Costs c = costs_of(1, false, s.block_dims);
+    double a = 0.0, b = 0.0;
+    std::vector<Group> x = one_each(decode, n, c, &a), y = shares(decode, n, per_cu, c, &b);
+    *t = std::min(a, b);
+    return a <= b ? x : y;
+  };
+  auto plan_prompts = [&](int n, std::vector<Tile>* tiles, double* t) {
+    std::vector<Group> best;
+    *t = 1e30;
+    const char* force = std::getenv("E4_FORCE");
+    for (int rw : {4, 2, 1}) {
+      const std::vector<Tile> x = prompt_tiles(rw);
+      if (rw < 4 && best.size() >= 4 * (std::size_t)n) break;  // (large tiles alone fill the device)
+      const Costs c = costs_of(rw, true, s.block_dims);
+      for (int mode = 0; mode < 3; ++mode) {
+        if (force && std::atoi(force) != rw * 10 + mode) continue;
+        double e = 0.0;
+        std::vector<Group> gr = mode == 0 ? whole(x, n, c, &e) : mode == 1 ? one_each(x, n, c, &e) : shares(x, n, per_cu, c, &e);
+        if (e < *t) {
+          *t = e;
+          best = std::move(gr);
+          *tiles = x;
+        }
+      }
+    }
+    return by_xcd(std::move(best));
+  };
+  std::vector<Group> dg, pg;
+  std::vector<Tile> pt;
+  if (!prompts) {
+    dg = plan_decode(slots, &time);
+  } else if (decode.empty()) {
+    pg = plan_prompts(slots, &pt, &time);
+  } else {
+    // both kinds: slots in proportion to the work
+    double d = 0.0, p = 0.0;
+    dg = plan_decode(slots, &d);
+    pg = plan_prompts(slots, &pt, &p);
+    const int n = std::max(1, std::min(slots - 1, (int)(slots * d / (d + p) + 0.5)));
+    dg = plan_decode(n, &d);
+    pg = plan_prompts(slots - n, &pt, &p);
   }
-  out.groups = (int)out.wg_first.size();
-  out.wg_first.push_back((int)out.items.size());
+  add(decode, dg, true);
+  add(pt, pg, false);
+  // A workgroup's first item has its index, its later ones follow the firsts.
+  out.groups = (int)all.size();
+  out.items.resize(all.size());
+  for (std::size_t i = 0; i < all.size(); ++i) {
+    std::size_t at = i;
+    for (std::size_t k = 0; k < all[i].size(); ++k) {
+      if (k) {
+        out.items[at].next = (int)out.items.size();
+        at = out.items.size();
+        out.items.emplace_back();
+      }
+      out.items[at] = all[i][k];
+    }
+  }
 }
 
 }  // namespace tge::plan

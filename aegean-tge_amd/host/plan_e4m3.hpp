@@ -11,14 +11,13 @@ namespace tge::plan {
 struct E4m3Lists {
   std::vector<E4m3Tile> tiles;
   bool page_twice = false;  // two sessions append into one page
-  std::vector<E4m3Item> items;
-  std::vector<int> wg_first;  // [groups + 1]
+  std::vector<E4m3Item> items;  // workgroup i starts with item i
   std::vector<E4m3Merge> merges;
   int groups = 0;
   int parts = 0;
 };
 
-// `slots`: workgroups that the device holds at once.
-void build_e4m3(const Step& s, int slots, E4m3Lists& out);
+// `cus` compute units, each holding `per_cu` workgroups at once.
+void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out);
 
 }  // namespace tge::plan
