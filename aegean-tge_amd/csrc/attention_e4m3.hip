@@ -46,11 +46,13 @@ struct E4m3Cfg {
   static_assert(4 * NB(1) * TP(1) == 16 && 2 * NB(2) * TP(2) == 16 && NB(4) * TP(4) == 16, "ring size");
 };
 
+constexpr int kE4m3Window = 1024;  // pages whose block numbers are in LDS at a time
+
 template <int W>
 struct E4m3Shared {
   alignas(16) char ring[E4m3Cfg<W>::RING];  // at a tile's end: the waves' accumulators
-  int ids[kE4m3ItemPages];                  // the item's pages: block numbers
-  alignas(8) uint32_t scales[kE4m3ItemPages];  // and their scale pairs
+  int ids[kE4m3Window];                  // of the item's pages: block numbers
+  alignas(8) uint32_t scales[kE4m3Window];  // and their scale pairs
   long out_at[kE4m3Rows];                   // element offset of each row in out
   float ml[2][4][32];                       // per wave: base, sum
   float sum[kE4m3Rows];
@@ -270,12 +272,54 @@ __device__ __forceinline__ int thread_here() {
   return t;
 }
 
-// Adds the pieces of J chunks of 4 dims a thread, K pieces in flight.
+// The states of a split tile's pieces become its output: the pieces' maxima
+// and sums are read at once and turned into weights in LDS, while the first
+// accumulators are on their way already; every thread adds J chunks of 4 dims,
+// K pieces in flight. The sums are in the pieces' order.
 template <int W, int J, int K>
-__device__ __forceinline__ void add_parts(const E4m3Attn& p, const E4m3Shared<W>& sh, const E4m3Merge& m,
-                                          __amdgpu_buffer_rsrc_t rs_o, __amdgpu_buffer_rsrc_t rs_ml,
-                                          const float2* ml, bool fits, int t) {
-  const int rows = m.rows, n = m.n_parts, chunks = rows * (W / 4);
+__device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh, const E4m3Item& it,
+                                            const E4m3Merge& m) {
+  const auto rs_o = make_rsrc(p.part_o, 0x7fffffff);
+  const auto rs_ml = make_rsrc(p.part_ml, 0x7fffffff);
+  const int t = thread_here(), rows = m.rows, n = m.n_parts, chunks = rows * (W / 4);
+  float2* const ml = reinterpret_cast<float2*>(sh.ring);  // [n][rows]: (base, sum), then (weight, -)
+  const bool fits = (size_t)n * rows * sizeof(float2) <= sizeof(sh.ring);  // else they are read where they are used
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  auto state = [&](int k, int r) __attribute__((always_inline)) {
+    return coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + k) * p.part_rows + r) * 8));
+  };
+  float4_t o[J][K];
+  auto load = [&](int i0, int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int idx = min(i0 + 256 * j, chunks - 1), r = idx / (W / 4), d4 = idx % (W / 4);
+#pragma unroll
+      for (int e = 0; e < K; ++e)
+        o[j][e] = coh_load4(rs_o, (uint32_t)((((size_t)(m.first_part + min(k0 + e, n - 1)) * p.part_rows + r) * W + 4 * d4) * 4));
+    }
+  };
+  if (fits) {
+#pragma unroll 1
+    for (int i = t; i < n * rows; i += 256) ml[i] = state(i / rows, i % rows);
+  }
+  load(t, 0);
+  // (LDS alone is ordered: the accumulators stay in flight)
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if (t < rows) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) top = fmaxf(top, fits ? ml[k * rows + t].x : state(k, t).x);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float2 v = fits ? ml[k * rows + t] : state(k, t);
+      const float w = v.x == -INFINITY ? 0.0f : pow2i(v.x - top);
+      sum += w * v.y;
+      if (fits) ml[k * rows + t].x = w;
+    }
+    sh.base[t] = top;
+    sh.sum[t] = sum;
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll 1
   for (int i0 = t; i0 < chunks; i0 += 256 * J) {
     float4_t acc[J];
@@ -283,14 +327,7 @@ __device__ __forceinline__ void add_parts(const E4m3Attn& p, const E4m3Shared<W>
     for (int j = 0; j < J; ++j) acc[j] = float4_t{0, 0, 0, 0};
 #pragma unroll 1
     for (int k0 = 0; k0 < n; k0 += K) {
-      float4_t o[J][K];
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int idx = min(i0 + 256 * j, chunks - 1), r = idx / (W / 4), d4 = idx % (W / 4);
-#pragma unroll
-        for (int e = 0; e < K; ++e)
-          o[j][e] = coh_load4(rs_o, (uint32_t)((((size_t)(m.first_part + min(k0 + e, n - 1)) * kE4m3Rows + r) * W + 4 * d4) * 4));
-      }
+      if (i0 != t || k0 != 0) load(i0, k0);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int r = min(i0 + 256 * j, chunks - 1) / (W / 4);
@@ -300,8 +337,7 @@ __device__ __forceinline__ void add_parts(const E4m3Attn& p, const E4m3Shared<W>
           if (fits) {
             w = ml[min(k0 + e, n - 1) * rows + r].x;
           } else {
-            const float x =
-                coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + min(k0 + e, n - 1)) * kE4m3Rows + r) * 8)).x;
+            const float x = state(min(k0 + e, n - 1), r).x;
             w = x == -INFINITY ? 0.0f : pow2i(x - sh.base[r]);
           }
           if (k0 + e < n) acc[j] += o[j][e] * w;
@@ -318,48 +354,6 @@ __device__ __forceinline__ void add_parts(const E4m3Attn& p, const E4m3Shared<W>
       }
     }
   }
-}
-
-// The states of a split tile's pieces become its output: the pieces' maxima
-// and sums are read at once and turned into weights in LDS, then every thread
-// adds its chunks. The sums are in the pieces' order.
-template <int W>
-__device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh, const E4m3Item& it,
-                                            const E4m3Merge& m) {
-  const auto rs_o = make_rsrc(p.part_o, 0x7fffffff);
-  const auto rs_ml = make_rsrc(p.part_ml, 0x7fffffff);
-  const int t = thread_here(), rows = m.rows, n = m.n_parts;
-  float2* const ml = reinterpret_cast<float2*>(sh.ring);  // [n][rows]: (base, sum), then (weight, -)
-  const bool fits = (size_t)n * rows * sizeof(float2) <= sizeof(sh.ring);  // else they are read where they are used
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  auto state = [&](int k, int r) __attribute__((always_inline)) {
-    return coh_load2(rs_ml, (uint32_t)(((size_t)(m.first_part + k) * kE4m3Rows + r) * 8));
-  };
-  if (fits) {
-#pragma unroll 4
-    for (int i = t; i < n * rows; i += 256) ml[i] = state(i / rows, i % rows);
-    __syncthreads();
-  }
-  if (t < rows) {
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) top = fmaxf(top, fits ? ml[k * rows + t].x : state(k, t).x);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float2 v = fits ? ml[k * rows + t] : state(k, t);
-      const float w = v.x == -INFINITY ? 0.0f : pow2i(v.x - top);
-      sum += w * v.y;
-      if (fits) ml[k * rows + t].x = w;
-    }
-    sh.base[t] = top;
-    sh.sum[t] = sum;
-  }
-  __syncthreads();
-  // (16 loads in flight either way)
-  if (rows * (W / 4) <= 256)
-    add_parts<W, 1, 16>(p, sh, m, rs_o, rs_ml, ml, fits, t);
-  else
-    add_parts<W, 4, 4>(p, sh, m, rs_o, rs_ml, ml, fits, t);
   if (t == 0) __hip_atomic_store(p.counters + it.merge, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -373,47 +367,14 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave % RW, ks = wave / RW;
   const int c = lane & 31, h = lane >> 5;
-  const int npages = it.page_end - it.page_begin;
-  const int ntiles = (npages + TP - 1) / TP;
-  const int turns = (ntiles + KS - 1) / KS;
-
-  // ---- the item's block numbers and rows
-  // (to a whole number of tiles: pages past the range repeat the last one,
-  // whose positions there no row sees)
-  const int padded = (npages + 7) & ~7;
-  for (int j = threadIdx.x; j < padded; j += 256)
-    sh.ids[j] = p.tables[it.table_off + it.page_begin + min(j, npages - 1)] * p.kv_heads + it.kv_head;
+  // (the first pages' ids are on their way while the rows are set up)
+  const int first_id = p.tables[it.table_off + min(it.page_begin + (int)threadIdx.x, it.page_end - 1)];
+  // ---- the item's rows
   if ((int)threadIdx.x < it.rows) {
     const int r = it.row0 + threadIdx.x, query = r / p.group;
     sh.out_at[threadIdx.x] = (long)(it.q_row + query) * p.out_stride +
                              (long)(it.kv_head * p.group + r - query * p.group) * p.dims;
   }
-  __syncthreads();
-
-  char* const ring = sh.ring + ks * NB * TP * C::BLOCK;
-  // Tile `turn * KS + ks` of the item into its slot (a group past the item's
-  // last tile copies that one again).
-  auto fetch = [&](int turn) __attribute__((always_inline)) {
-    char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
-    const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
-    int n[MINE];
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) n[i] = sh.ids[j0 + i];
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const int block = __builtin_amdgcn_readfirstlane(n[i]);
-      if (it.once)
-        fetch_block<W, kPageLoadPolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
-      else
-        fetch_block<W, kPageReusePolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
-    }
-  };
-  constexpr int AHEAD = RW == 1 ? NB : NB - 1;  // tiles copied before the first is used
-#pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
-    if (k < turns) fetch(k);
-  for (int j = threadIdx.x; j < padded; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
-
   E4m3Rows<W> x;
   {
     // f16 rows enter the products as they are and the scores are scaled
@@ -447,40 +408,80 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
 #pragma unroll
       for (int e = 0; e < 16; ++e) x.o[i][e] = 0.0f;
   }
-  __syncthreads();  // scales are in LDS
 
-  for (int turn = 0; turn < turns; ++turn) {
-    char* const slot = ring + (turn % NB) * TP * C::BLOCK;
-    const int j0 = (turn * KS + ks) * TP;
-    const int page = it.page_begin + j0;
-    if constexpr (RW == 1) {
-      // The wave's own ring: once a tile's codes are in registers its slot
-      // takes the tile NB turns on, so NB tiles are in flight while one is
-      // worked on.
-      if (turn + 1 < turns)
-        wait_vmcnt<(NB - 1) * LOADS>();
-      else
-        wait_vmcnt<0>();
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      const int j = min(j0, padded - TP);
-      E4m3Codes<W> codes;
-      codes.read(slot, sh.scales + j, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (turn + NB < turns) fetch(turn + NB);
-      if (j0 < npages && page * 16 <= x.last_lim) x.pair(codes, page, lane);
-    } else {
-      wait_vmcnt_pages<NB - 2, LOADS>(min(NB - 2, turns - 1 - turn));
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (turn + NB - 1 < turns) fetch(turn + NB - 1);
+  char* const ring = sh.ring + ks * NB * TP * C::BLOCK;
+  for (int begin = it.page_begin; begin < it.page_end; begin += kE4m3Window) {
+    const int npages = min(it.page_end - begin, kE4m3Window);
+    const int ntiles = (npages + TP - 1) / TP;
+    const int turns = (ntiles + KS - 1) / KS;
+    // The pages' block numbers, to a whole number of tiles: pages past the
+    // range repeat the last one, whose positions there no row sees.
+    const int padded = (npages + 7) & ~7;
+    for (int j = threadIdx.x; j < padded; j += 256) {
+      const bool have = begin == it.page_begin && j < 256;
+      const int id = have ? first_id : p.tables[it.table_off + begin + min(j, npages - 1)];
+      sh.ids[j] = id * p.kv_heads + it.kv_head;
+    }
+    __syncthreads();
+
+    // Tile `turn * KS + ks` of the item into its slot (a group past the item's
+    // last tile copies that one again).
+    auto fetch = [&](int turn) __attribute__((always_inline)) {
+      char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
+      const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
+      int n[MINE];
 #pragma unroll
-      for (int b = 0; b < TP; b += 2) {
-        if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
-          E4m3Codes<W> codes;
-          codes.read(slot + b * C::BLOCK, sh.scales + j0 + b, lane);
-          x.pair(codes, page + b, lane);
+      for (int i = 0; i < MINE; ++i) n[i] = sh.ids[j0 + i];
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int block = __builtin_amdgcn_readfirstlane(n[i]);
+        if (it.once)
+          fetch_block<W, kPageLoadPolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
+        else
+          fetch_block<W, kPageReusePolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
+      }
+    };
+    constexpr int AHEAD = RW == 1 ? NB : NB - 1;  // tiles copied before the first is used
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (k < turns) fetch(k);
+    for (int j = threadIdx.x; j < padded; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
+    __syncthreads();  // scales are in LDS
+
+    for (int turn = 0; turn < turns; ++turn) {
+      char* const slot = ring + (turn % NB) * TP * C::BLOCK;
+      const int j0 = (turn * KS + ks) * TP;
+      const int page = begin + j0;
+      if constexpr (RW == 1) {
+        // The wave's own ring: once a tile's codes are in registers its slot
+        // takes the tile NB turns on, so NB tiles are in flight while one is
+        // worked on.
+        if (turn + 1 < turns)
+          wait_vmcnt<(NB - 1) * LOADS>();
+        else
+          wait_vmcnt<0>();
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        const int j = min(j0, padded - TP);
+        E4m3Codes<W> codes;
+        codes.read(slot, sh.scales + j, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (turn + NB < turns) fetch(turn + NB);
+        if (j0 < npages && page * 16 <= x.last_lim) x.pair(codes, page, lane);
+      } else {
+        wait_vmcnt_pages<NB - 2, LOADS>(min(NB - 2, turns - 1 - turn));
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (turn + NB - 1 < turns) fetch(turn + NB - 1);
+#pragma unroll
+        for (int b = 0; b < TP; b += 2) {
+          if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
+            E4m3Codes<W> codes;
+            codes.read(slot + b * C::BLOCK, sh.scales + j0 + b, lane);
+            x.pair(codes, page + b, lane);
+          }
         }
       }
     }
+    if (begin + kE4m3Window < it.page_end) __syncthreads();  // every wave has left the window's tables
   }
 
   // ---- the groups' states become one: common bases, sums, accumulators
@@ -538,8 +539,8 @@ __device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh
         store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
                    sum > 0.0f || sum != sum ? div4(acc, sum) : float4_t{0, 0, 0, 0});
     } else {
-      coh_store4(rs_o, (uint32_t)((((size_t)it.part * kE4m3Rows + r) * W + 4 * d4) * 4), acc);
-      if (d4 == 0) coh_store2(rs_ml, (uint32_t)(((size_t)it.part * kE4m3Rows + r) * 8), sh.base[r], sh.sum[r]);
+      coh_store4(rs_o, (uint32_t)((((size_t)it.part * p.part_rows + r) * W + 4 * d4) * 4), acc);
+      if (d4 == 0) coh_store2(rs_ml, (uint32_t)(((size_t)it.part * p.part_rows + r) * 8), sh.base[r], sh.sum[r]);
     }
   }
   if (it.part >= 0) {
@@ -551,7 +552,12 @@ __device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh
       sh.flag = __hip_atomic_fetch_add(p.counters + it.merge, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                 m.n_parts - 1;
     __syncthreads();
-    if (sh.flag) merge_parts<W>(p, sh, it, m);
+    if (sh.flag) {
+      if (m.rows * (W / 4) <= 256)
+        merge_parts<W, 1, 16>(p, sh, it, m);
+      else
+        merge_parts<W, 4, 4>(p, sh, it, m);
+    }
   }
   __syncthreads();  // the shared state is free for the next item
 }

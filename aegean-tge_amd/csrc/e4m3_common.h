@@ -95,7 +95,6 @@ struct E4m3Merge {
   int pad[2];
 };
 
-constexpr int kE4m3ItemPages = 1024;  // pages of an item (its page table sits in LDS)
-constexpr int kE4m3Rows = 128;        // rows of a partial slot
+constexpr int kE4m3Rows = 128;  // rows of a tile at most
 
 }  // namespace tge

@@ -52,8 +52,9 @@ struct E4m3Attn {
   int group;
   int dims;
   float scale_log2;  // softmax scale * log2(e)
-  float* part_o;     // [parts][kE4m3Rows][width]
-  float* part_ml;    // [parts][kE4m3Rows][2]
+  float* part_o;     // [parts][part_rows][width]
+  float* part_ml;    // [parts][part_rows][2]
+  int part_rows;
 };
 
 struct E4m3Gather {

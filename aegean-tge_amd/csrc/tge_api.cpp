@@ -539,7 +539,7 @@ int plan_e4m3(tge_batch* b, hipStream_t hs) {
   E4m3Plan& e = b->e4;
   tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
   const auto& L = e.lists;
-  if ((size_t)L.parts * tge::kE4m3Rows * st.block_dims * sizeof(float) > 0x7fffffffu)
+  if ((size_t)L.parts * L.part_rows * st.block_dims * sizeof(float) > 0x7fffffffu)
     return fail(TGE_ERR_CAPACITY, "batch_plan: the step's partial states exceed 2 GiB");
   const size_t o_rows = align_up(st.tables.size() * sizeof(int));
   e.off_tiles = align_up(o_rows + st.rows.size() * sizeof(tge::RowRec));
@@ -561,7 +561,7 @@ int plan_e4m3(tge_batch* b, hipStream_t hs) {
   if (s != TGE_OK) return s;
   b->off_tables = 0;
   b->off_rows = o_rows;
-  const size_t rows = (size_t)std::max(L.parts, 1) * tge::kE4m3Rows;
+  const size_t rows = (size_t)std::max(L.parts, 1) * L.part_rows;
   s = e.part_o.reserve(g_mem, rows * st.block_dims * sizeof(float), hs);
   if (s == TGE_OK) s = e.part_ml.reserve(g_mem, rows * 2 * sizeof(float), hs);
   if (s != TGE_OK) return s;
@@ -972,6 +972,7 @@ int attention_params_e4m3(const tge_batch* b, const tge_kv_pool* p, int layer, c
   x.scale_log2 = (float)(1.4426950408889634 * (a.scale > 0.0f ? (double)a.scale : 1.0 / std::sqrt((double)hd)));
   x.part_o = reinterpret_cast<float*>(e.part_o.dev);
   x.part_ml = reinterpret_cast<float*>(e.part_ml.dev);
+  x.part_rows = e.lists.part_rows;
   return TGE_OK;
 }
 

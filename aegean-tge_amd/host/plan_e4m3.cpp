@@ -2,7 +2,6 @@
 #include "plan_e4m3.hpp"
 
 #include <algorithm>
-#include <cstdlib>
 #include <utility>
 
 namespace tge::plan {
@@ -24,64 +23,70 @@ struct Piece {
 
 using Group = std::vector<Piece>;
 
-// Costs in microseconds of a workgroup while every slot is busy, fitted to
-// launches of 0.5 to 280 GFLOP with every tile size and way to cut.
+// Costs in microseconds of a workgroup while every slot is busy.
 struct Costs {
   double page;    // a page
   double start;   // an item's start and end
   double merge;   // a tile that is cut: its merge
-  double solo;    // cost of an item, relative, where most slots are idle
-  double spread;  // cost of a page, relative, in shares: neighbours are at different pages and share the L2 less
+  double solo;    // cost of a page, relative, where the compute unit's other slots are idle
+  double uneven;  // what the longest item adds to a launch, relative
   int grain;      // pages that the waves share out at a time
   int least;      // pages of a piece
+  int rounds;     // pieces at most, in slots
 
-  double time(double total, double longest, int slots, bool cut) const {
-    return std::max(total / slots + 0.3 * longest, solo * longest) + (cut ? merge : 0.0);
+  double time(double total, int pages, int slots, bool cut) const {
+    return std::max(total / slots + uneven * (pages * page + start), pages * page * solo + start) + (cut ? merge : 0.0);
   }
 };
 
 // A decode page is bound by HBM (4 KiB at 512 workgroups' shares of 5.6 TB/s),
 // a prompt page by the matrix cores and the exponentials; waves that share
-// their pages (a larger rw) pay less for the copies.
+// their pages (a larger rw) pay less for the copies. Fitted at 28/4 heads of
+// 128 dims, rw 1 / 2 / 4, us measured (by this model): 2048 tokens 61 / 52 / 51
+// (59 / 53 / 53), 512 behind 1536 25 / 32 / 47 (25 / 31 / 53), 1333 behind
+// 14003 uncut 363 / 388 / 431 (379 / 388 / 412), in four pieces 313 at rw 4.
 Costs costs_of(int rw, bool prompt, int width) {
   const double w = width / 128.0;
-  if (!prompt) return Costs{0.37 * w, 4.5, 4.0, 0.25, 1.0, 8, 32};
-  const double page = rw == 1 ? 0.155 : rw == 2 ? 0.32 : 0.45;
-  return Costs{page * w, 5.0, 6.0 + 2.0 * rw, 0.75, 1.35, rw == 1 ? 8 : 4, 32};
+  if (!prompt) return Costs{0.37 * w, 4.5, 4.0, 0.25, 0.05, 8, 32, 1};
+  const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
+  return Costs{page * w, 4.0, 6.0 + 2.0 * rw, 0.7, 0.25, rw == 1 ? 8 : 4, 32, 4};
 }
 
-// Each tile in equal pieces, a piece a group: the shortest pieces that fit.
-std::vector<Group> one_each(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
-  int most = 0;
-  for (const Tile& t : tiles) most = std::max(most, t.pages);
-  int lo = c.least, hi = std::max(most, c.least);
-  auto count = [&](int p) {
-    long long n = 0;
-    for (const Tile& t : tiles) n += ceil_div(t.pages, p);
-    return n;
-  };
-  hi = std::min(hi, kE4m3ItemPages);
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (count(mid) <= slots)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
+// Each tile in equal pieces of at most `len` pages, a piece a group.
+std::vector<Group> pieces(const std::vector<Tile>& tiles, int len, const Costs& c) {
   std::vector<Group> groups;
-  double longest = 0.0, total = 0.0;
-  bool cut = false;
   for (std::size_t i = 0; i < tiles.size(); ++i) {
-    const int n = ceil_div(tiles[i].pages, lo), len = ceil_div(ceil_div(tiles[i].pages, n), c.grain) * c.grain;
-    const int of = ceil_div(tiles[i].pages, len);
+    const int n = ceil_div(tiles[i].pages, len);
+    const int each = ceil_div(ceil_div(tiles[i].pages, n), c.grain) * c.grain, of = ceil_div(tiles[i].pages, each);
     for (int k = 0; k < of; ++k)
-      groups.push_back({Piece{(int)i, k * len, std::min((k + 1) * len, tiles[i].pages), k, of}});
-    longest = std::max(longest, std::min(len, tiles[i].pages) * c.page + c.start);
-    total += tiles[i].pages * c.page + of * c.start;
-    cut = cut || of > 1;
+      groups.push_back({Piece{(int)i, k * each, std::min((k + 1) * each, tiles[i].pages), k, of}});
   }
-  *time = c.time(total, longest, slots, cut);
   return groups;
+}
+
+// Of the piece lengths the one with the least time.
+int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
+  int most = 0, best = 0;
+  for (const Tile& t : tiles) most = std::max(most, t.pages);
+  *time = 1e30;
+  for (int len = ceil_div(most, c.grain) * c.grain;;) {
+    long long n = 0;
+    double total = 0.0;
+    for (const Tile& t : tiles) {
+      const int of = ceil_div(t.pages, len);
+      n += of;
+      total += t.pages * c.page + of * c.start;
+    }
+    if (best && n > (long long)slots * c.rounds) break;
+    const double t = c.time(total, std::min(len, most), slots, len < most);
+    if (t < *time) {
+      *time = t;
+      best = len;
+    }
+    len = std::min(len - c.grain, len * 15 / 16 / c.grain * c.grain);
+    if (len < c.least) break;
+  }
+  return best;
 }
 
 // The tiles end to end, cut into shares, a share a group. Workgroups that land
@@ -112,7 +117,6 @@ std::vector<Group> shares(const std::vector<Tile>& tiles, int slots, int per_cu,
         }
         int n = std::min(pages - begin, std::max(least, (int)((left - c.start) / c.page) / c.grain * c.grain));
         if (pages - begin - n < least) n = pages - begin;  // (no slivers)
-        n = std::min(n, kE4m3ItemPages);
         begin += n;
         left -= n * c.page + c.start;
         at.emplace_back(begin, (int)groups.size() - 1);
@@ -124,42 +128,56 @@ std::vector<Group> shares(const std::vector<Tile>& tiles, int slots, int per_cu,
     }
     if ((int)groups.size() <= slots) break;
   }
-  *time = c.spread * share + 0.3 * c.start + (cut ? c.merge : 0.0);
+  *time = share + 0.5 * c.start + (cut ? c.merge : 0.0);
   return groups;
 }
 
-// Whole tiles, the longest first (more tiles than slots: the device takes the
-// next one as a slot falls free).
-std::vector<Group> whole(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
-  std::vector<std::size_t> order(tiles.size());
-  for (std::size_t i = 0; i < order.size(); ++i) order[i] = i;
-  std::stable_sort(order.begin(), order.end(),
-                   [&](std::size_t a, std::size_t b) { return tiles[a].pages > tiles[b].pages; });
-  std::vector<Group> groups(tiles.size());
-  double longest = 0.0, total = 0.0;
-  for (std::size_t k = 0; k < order.size(); ++k) {
-    const int pages = tiles[order[k]].pages, of = ceil_div(pages, kE4m3ItemPages);
-    for (int p = 0; p < of; ++p)
-      groups[k].push_back(Piece{(int)order[k], p * kE4m3ItemPages, std::min((p + 1) * kE4m3ItemPages, pages), p, of});
-    const double t = pages * c.page + of * c.start;
-    longest = std::max(longest, t);
-    total += t;
+// Workgroup b runs on XCD b mod 8, each with an L2 of its own and slots / 8
+// workgroups: the pieces of one (session, KV head), which read the same pages,
+// go to few XCDs, every XCD gets about the same work, the longest first. (8192
+// tokens, 28/4 heads of 128 dims: 782 us with the longest of all heads first on
+// every XCD.)
+std::vector<Group> by_xcd(const std::vector<Tile>& tiles, std::vector<Group> groups, int slots) {
+  constexpr int X = 8;
+  const std::size_t n = groups.size();
+  std::vector<int> pages(n);
+  std::vector<std::size_t> order(n);
+  int streams = 0;
+  std::vector<int> stream(n);
+  for (std::size_t i = 0; i < n; ++i) {
+    const Tile& t = tiles[(std::size_t)groups[i][0].tile];
+    if (i > 0) {
+      const Tile& u = tiles[(std::size_t)groups[i - 1][0].tile];
+      streams += t.session != u.session || t.kv_head != u.kv_head;
+    }
+    stream[i] = streams;
+    for (const Piece& p : groups[i]) pages[i] += p.end - p.begin;
+    order[i] = i;
   }
-  *time = c.time(total, longest, slots, false);
-  return groups;
-}
-
-// Workgroup b runs on XCD b mod 8, each with an L2 of its own: neighbours in
-// the list, which read the same pages, go to one XCD.
-std::vector<Group> by_xcd(std::vector<Group> groups) {
-  const std::size_t n = groups.size(), x = 8;
+  ++streams;
+  std::stable_sort(order.begin(), order.end(), [&](std::size_t a, std::size_t b) { return pages[a] > pages[b]; });
+  std::vector<std::size_t> list[X];
+  long long load[X] = {};
+  for (std::size_t i : order) {
+    // the stream's own XCDs, then any with room
+    const int lo = stream[i] * X / streams, hi = std::max(lo + 1, ((stream[i] + 1) * X + streams - 1) / streams);
+    int best = -1;
+    for (int x = lo; x < std::min(hi, X); ++x)
+      if (list[x].size() < (n - x + X - 1) / X && (best < 0 || load[x] < load[best])) best = x;
+    for (int x = 0; best < 0 && x < X; ++x)
+      if (list[x].size() < (n - x + X - 1) / X) best = x;
+    list[best].push_back(i);
+    load[best] += pages[i];
+  }
+  // Where all groups are resident at once, the second workgroup of a compute
+  // unit is short where the first is long.
+  for (auto& l : list) {
+    const std::size_t half = (std::size_t)slots / (2 * X);
+    if (n <= (std::size_t)slots && l.size() > half) std::reverse(l.begin() + (long)half, l.end());
+  }
   std::vector<Group> out;
   out.reserve(n);
-  for (std::size_t i = 0; i < n; ++i) {
-    // chunk i % 8 starts after the chunks before it (the first n % 8 hold one more)
-    const std::size_t chunk = i % x, per = n / x, more = n % x;
-    out.push_back(std::move(groups[chunk * per + std::min(chunk, more) + i / x]));
-  }
+  for (std::size_t i = 0; i < n; ++i) out.push_back(std::move(groups[list[i % X][i / X]]));
   return out;
 }
 
@@ -171,6 +189,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
   out.items.clear();
   out.merges.clear();
   out.groups = out.parts = 0;
+  out.part_rows = 32;
   out.page_twice = false;
 
   // ---- append: the pages that new rows fall into
@@ -230,6 +249,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
         int& m = merge[(std::size_t)p.tile];
         if (p.of > 1 && m < 0) {
           m = (int)out.merges.size();
+          out.part_rows = std::max(out.part_rows, 32 * t.rw);
           out.merges.push_back(E4m3Merge{out.parts, p.of, t.rows, t.row0, t.kv_head, r.q_row, {}});
           out.parts += p.of;
         }
@@ -244,30 +264,27 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
   auto plan_decode = [&](int n, double* t) {
     const Costs c = costs_of(1, false, s.block_dims);
     double a = 0.0, b = 0.0;
-    std::vector<Group> x = one_each(decode, n, c, &a), y = shares(decode, n, per_cu, c, &b);
+    const int len = piece_length(decode, n, c, &a);
+    std::vector<Group> y = shares(decode, n, per_cu, c, &b);
     *t = std::min(a, b);
-    return a <= b ? x : y;
+    return a <= b ? pieces(decode, len, c) : y;
   };
   auto plan_prompts = [&](int n, std::vector<Tile>* tiles, double* t) {
     std::vector<Group> best;
     *t = 1e30;
-    const char* force = std::getenv("E4_FORCE");
     for (int rw : {4, 2, 1}) {
-      const std::vector<Tile> x = prompt_tiles(rw);
+      std::vector<Tile> x = prompt_tiles(rw);
       if (rw < 4 && best.size() >= 4 * (std::size_t)n) break;  // (large tiles alone fill the device)
       const Costs c = costs_of(rw, true, s.block_dims);
-      for (int mode = 0; mode < 3; ++mode) {
-        if (force && std::atoi(force) != rw * 10 + mode) continue;
-        double e = 0.0;
-        std::vector<Group> gr = mode == 0 ? whole(x, n, c, &e) : mode == 1 ? one_each(x, n, c, &e) : shares(x, n, per_cu, c, &e);
-        if (e < *t) {
-          *t = e;
-          best = std::move(gr);
-          *tiles = x;
-        }
+      double e = 0.0;
+      const int len = piece_length(x, n, c, &e);
+      if (e < *t) {
+        *t = e;
+        best = pieces(x, len, c);
+        *tiles = std::move(x);
       }
     }
-    return by_xcd(std::move(best));
+    return by_xcd(*tiles, std::move(best), n);
   };
   std::vector<Group> dg, pg;
   std::vector<Tile> pt;

@@ -14,7 +14,8 @@ struct E4m3Lists {
   std::vector<E4m3Item> items;  // workgroup i starts with item i
   std::vector<E4m3Merge> merges;
   int groups = 0;
-  int parts = 0;
+  int parts = 0;      // partial states
+  int part_rows = 32; // rows of each
 };
 
 // `cus` compute units, each holding `per_cu` workgroups at once.
