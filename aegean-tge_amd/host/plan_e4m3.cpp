@@ -34,22 +34,30 @@ struct Costs {
   int least;      // pages of a piece
   int rounds;     // pieces at most, in slots
 
-  double time(double total, int pages, int slots, bool cut) const {
-    return std::max(total / slots + uneven * (pages * page + start), pages * page * solo + start) + (cut ? merge : 0.0);
+  // `n` items of `total` in all, the longest of `pages`.
+  double time(double total, long long n, int pages, int slots, bool cut) const {
+    double t = std::max(total / slots + uneven * (pages * page + start), pages * page * solo + start);
+    // (a last round of few items runs faster, but a round it is)
+    const long long full = n / slots;
+    const double last = (double)n / slots - full;
+    if (full > 0) t = std::max(t, total / n * (full + (last == 0.0 ? 0.0 : last <= 0.5 ? 0.6 : 1.0)));
+    return t + (cut ? merge : 0.0);
   }
 };
 
-// A decode page is bound by HBM (4 KiB at 512 workgroups' shares of 5.6 TB/s),
-// a prompt page by the matrix cores and the exponentials; waves that share
-// their pages (a larger rw) pay less for the copies. Fitted at 28/4 heads of
-// 128 dims, rw 1 / 2 / 4, us measured (by this model): 2048 tokens 61 / 52 / 51
-// (59 / 53 / 53), 512 behind 1536 25 / 32 / 47 (25 / 31 / 53), 1333 behind
-// 14003 uncut 363 / 388 / 431 (379 / 388 / 412), in four pieces 313 at rw 4.
-Costs costs_of(int rw, bool prompt, int width) {
-  const double w = width / 128.0;
-  if (!prompt) return Costs{0.37 * w, 4.5, 4.0, 0.25, 0.05, 8, 32, 1};
+// A decode page is bound by HBM (a slot's share of 5.6 TB/s), a prompt page by
+// the matrix cores and the exponentials; waves that share their pages (a larger
+// rw) pay less for the copies. Fitted at 28/4 heads of 128 dims, rw 1 / 2 / 4,
+// us measured (by this model): 2048 tokens 61 / 52 / 51 (59 / 53 / 53), 512
+// behind 1536 25 / 32 / 47 (25 / 31 / 53), 1333 behind 14003 uncut 363 / 388 /
+// 431 (379 / 406 / 412), at rw 4 in three, four or five pieces a tile 335 / 313
+// / 327 (349 / 347 / 333). In 256-dim blocks a compute unit holds one workgroup.
+Costs costs_of(int rw, bool prompt, int width, int slots) {
+  if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 4.0, 0.25, 0.05, 8, 32, 1};
   const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
-  return Costs{page * w, 4.0, 6.0 + 2.0 * rw, 0.7, 0.25, rw == 1 ? 8 : 4, 32, 4};
+  const int grain = rw == 1 ? 8 : 4;
+  if (width > 128) return Costs{1.75 * page, 6.0, 6.0 + 4.0 * rw, 1.0, 0.25, grain, 32, 4};
+  return Costs{page * width / 128.0, 4.0, 6.0 + 2.0 * rw, 0.7, 0.25, grain, 32, 4};
 }
 
 // Each tile in equal pieces of at most `len` pages, a piece a group.
@@ -78,7 +86,7 @@ int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, doub
       total += t.pages * c.page + of * c.start;
     }
     if (best && n > (long long)slots * c.rounds) break;
-    const double t = c.time(total, std::min(len, most), slots, len < most);
+    const double t = c.time(total, n, std::min(len, most), slots, len < most);
     if (t < *time) {
       *time = t;
       best = len;
@@ -262,7 +270,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
 
   double time = 0.0;
   auto plan_decode = [&](int n, double* t) {
-    const Costs c = costs_of(1, false, s.block_dims);
+    const Costs c = costs_of(1, false, s.block_dims, slots);
     double a = 0.0, b = 0.0;
     const int len = piece_length(decode, n, c, &a);
     std::vector<Group> y = shares(decode, n, per_cu, c, &b);
@@ -275,7 +283,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
     for (int rw : {4, 2, 1}) {
       std::vector<Tile> x = prompt_tiles(rw);
       if (rw < 4 && best.size() >= 4 * (std::size_t)n) break;  // (large tiles alone fill the device)
-      const Costs c = costs_of(rw, true, s.block_dims);
+      const Costs c = costs_of(rw, true, s.block_dims, slots);
       double e = 0.0;
       const int len = piece_length(x, n, c, &e);
       if (e < *t) {
