@@ -69,10 +69,15 @@ __device__ __forceinline__ void store_row8(const float (&x)[8], void* row, long 
   }
 }
 
+// Eight floats of a table or bias from index `at` (a multiple of 8).
+__device__ __forceinline__ void load_f8(float (&x)[8], const float* p, long at) { load_row8<TGE_ROWS_F32>(x, p, at); }
+
 __device__ __forceinline__ void add8(float (&x)[8], const float* bias, int at) {
   if (!bias) return;
+  float b[8];
+  load_f8(b, bias, at);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], bias[at + i]);
+  for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], b[i]);
 }
 
 // One output of the rotation, l*c - h*s or l*s + h*c, with the second product
@@ -118,11 +123,32 @@ __device__ __forceinline__ void rotated_run(float (&x)[8], const E4m3Append& p, 
   load_row8<TYPE>(y, rows, base + other);
   add8(x, bias, head_at + d0);
   add8(y, bias, head_at + other);
-  const float* c = p.rope_cos + (long)pos * half + f;
-  const float* s = p.rope_sin + (long)pos * half + f;
+  float c[8], s[8];
+  load_f8(c, p.rope_cos, (long)pos * half + f);
+  load_f8(s, p.rope_sin, (long)pos * half + f);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     x[i] = low ? rot(x[i], c[i], y[i], -s[i], p.rope_fma != 0) : rot(y[i], s[i], x[i], c[i], p.rope_fma != 0);
+}
+
+// A run of 8 low dims (from f) and its partners, turned together.
+template <int TYPE>
+__device__ __forceinline__ void rotated_pair(float (&l)[8], float (&h)[8], const E4m3Append& p, const void* rows,
+                                             long base, const float* bias, int head_at, int f, int pos) {
+  const int half = p.dims >> 1;
+  float c[8], s[8];
+  load_row8<TYPE>(l, rows, base + f);
+  load_row8<TYPE>(h, rows, base + f + half);
+  load_f8(c, p.rope_cos, (long)pos * half + f);
+  load_f8(s, p.rope_sin, (long)pos * half + f);
+  add8(l, bias, head_at + f);
+  add8(h, bias, head_at + f + half);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = rot(l[i], c[i], h[i], -s[i], p.rope_fma != 0);
+    h[i] = rot(l[i], s[i], h[i], c[i], p.rope_fma != 0);
+    l[i] = a;
+  }
 }
 
 template <int TYPE, int W, bool ROPE>
@@ -148,12 +174,23 @@ __device__ __forceinline__ void append_part(const E4m3Append& p, char* stage, co
     for (int u = 0; u < U; ++u) was[u] = *reinterpret_cast<const u32x4_t*>(dst + u * 1024 + lane * 16);
   }
   float x[U][2][8];
-  float most = 0.0f;
+  // (heads as wide as their blocks of 128 or 256 dims hold a dim's partner in
+  // the same lane: one load each)
+  const bool paired = ROPE && U > 1 && part == 0 && p.dims == W;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int d0 = 64 * u + 16 * m + 8 * r;
+      if (paired) {
+        if (u >= U / 2) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][r][i] = x[(u + U / 2) % U][r][i] = 0.0f;
+        if (live)
+          rotated_pair<TYPE>(x[u][r], x[(u + U / 2) % U][r], p, rows, base, bias, h * p.dims, d0,
+                             t.pos + slot - t.slot);
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[u][r][i] = 0.0f;
       if (live && d0 < p.dims) {
@@ -164,10 +201,15 @@ __device__ __forceinline__ void append_part(const E4m3Append& p, char* stage, co
           if (ROPE) add8(x[u][r], bias, h * p.dims + d0);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[u][r][i]));  // (a NaN does not count)
     }
   }
+  float most = 0.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[u][r][i]));  // (a NaN does not count)
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off));
   const int need = e4m3_exponent(__float_as_uint(most));
@@ -228,37 +270,25 @@ template <int TYPE, int W, bool ROPE>
 __global__ __launch_bounds__(256) void kv_append_e4m3_kernel(E4m3Append p, int kv_groups) {
   __shared__ __align__(16) char stage[4][16 * W];
   if (ROPE && (int)blockIdx.x >= kv_groups) {
-    const int per_head = p.dims >> 4;
-    const long id = (long)(blockIdx.x - kv_groups) * 256 + threadIdx.x;
-    const long total = (long)p.n_rows * p.q_heads * per_head;
-    if (id >= total) return;
+    const uint32_t per_head = (uint32_t)p.dims >> 4;
+    const uint32_t id = (blockIdx.x - kv_groups) * 256u + threadIdx.x;
+    if (id >= (uint32_t)p.n_rows * p.q_heads * per_head) return;
     const int f = (int)(id % per_head) * 8;
-    const long rest = id / per_head;
+    const uint32_t rest = id / per_head;
     const int head = (int)(rest % p.q_heads), row = (int)(rest / p.q_heads);
-    const int half = p.dims >> 1;
-    const long at = (long)row * p.q_stride + (long)head * p.dims + f;
-    float l[8], h[8], a[8], b[8];
-    load_row8<TYPE>(l, p.q, at);
-    load_row8<TYPE>(h, p.q, at + half);
-    add8(l, p.q_bias, head * p.dims + f);
-    add8(h, p.q_bias, head * p.dims + f + half);
-    const long tab = (long)p.rows[row].pos * half + f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = p.rope_cos[tab + i], s = p.rope_sin[tab + i];
-      a[i] = rot(l[i], c, h[i], -s, p.rope_fma != 0);
-      b[i] = rot(l[i], s, h[i], c, p.rope_fma != 0);
-    }
+    float l[8], h[8];
+    rotated_pair<TYPE>(l, h, p, p.q, (long)row * p.q_stride + (long)head * p.dims, p.q_bias, head * p.dims, f,
+                       p.rows[row].pos);
     const long to = (long)row * p.q_out_stride + (long)head * p.dims + f;
-    store_row8<TYPE>(a, p.q_out, to);
-    store_row8<TYPE>(b, p.q_out, to + half);
+    store_row8<TYPE>(l, p.q_out, to);
+    store_row8<TYPE>(h, p.q_out, to + (p.dims >> 1));
     return;
   }
   const int wave = threadIdx.x >> 6;
-  const long unit = (long)blockIdx.x * 4 + wave;
-  if (unit >= (long)p.n_tiles * p.kv_heads * 2) return;  // whole waves
+  const uint32_t unit = blockIdx.x * 4u + wave;
+  if (unit >= (uint32_t)p.n_tiles * p.kv_heads * 2u) return;  // whole waves
   const int part = (int)(unit & 1);
-  const long rest = unit >> 1;
+  const uint32_t rest = unit >> 1;
   append_part<TYPE, W, ROPE>(p, stage[wave], p.tiles[rest / p.kv_heads], (int)(rest % p.kv_heads), part,
                              threadIdx.x & 63);
 }
@@ -286,7 +316,7 @@ hipError_t launch_append_type(const E4m3Append& p, hipStream_t stream) {
   const long kv_groups = (waves + 3) / 4;
   const long q_lanes = ROPE && p.q ? (long)p.n_rows * p.q_heads * (p.dims >> 4) : 0;
   const long groups = kv_groups + (q_lanes + 255) / 256;
-  if (groups > 0x7fffffff) return hipErrorInvalidValue;
+  if (groups > 0x7fffffff || waves > 0x7fffffff || q_lanes > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((unsigned)groups);
   if (p.width == 64)
     kv_append_e4m3_kernel<TYPE, 64, ROPE><<<grid, 256, 0, stream>>>(p, (int)kv_groups);

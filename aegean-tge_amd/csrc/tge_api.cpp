@@ -887,6 +887,9 @@ int append_e4m3(const tge_batch* b, tge_kv_pool* p, int layer, const tge_append_
   if (rope) {
     if (!a.rope_cos || !a.rope_sin) return fail(TGE_ERR_INVALID, std::string(who) + ": one rotary table without the other");
     if (hd % 16 != 0) return fail(TGE_ERR_INVALID, std::string(who) + ": head_dim must be a multiple of 16 to rotate");
+    for (const float* t : {a.rope_cos, a.rope_sin, a.q_bias, a.k_bias, a.v_bias})
+      if (reinterpret_cast<uintptr_t>(t) % 16 != 0)
+        return fail(TGE_ERR_INVALID, std::string(who) + ": tables and biases must be 16-byte aligned");
     if (a.q && !a.q_out) return fail(TGE_ERR_INVALID, std::string(who) + ": q without q_out");
     if (!a.q && a.q_out) return fail(TGE_ERR_INVALID, std::string(who) + ": q_out without q");
     if (a.q) {

@@ -351,8 +351,8 @@ int tge_batch_attention(const tge_batch* batch, const tge_kv_pool* pool,
  *
  * The two calls below take rows of fp32, f16 or bf16 with a stride, such as
  * slices of one projection's output: `*_stride` elements lie between rows (0:
- * none lie between them). Bases are 16-byte aligned and strides multiples of
- * 16 bytes. The fp32 calls on such a pool (tge_kv_append, tge_kv_append_rope,
+ * none lie between them). Bases (rotary tables and biases too) are 16-byte
+ * aligned and strides multiples of 16 bytes. The fp32 calls on such a pool (tge_kv_append, tge_kv_append_rope,
  * tge_decode_attention, tge_decode_step, tge_prefill_attention,
  * tge_batch_attention, the driver) are the same kernels with fp32 rows.
  * tge_decode_attention_static, tge_attention_group and a static sparse subset

@@ -490,6 +490,7 @@ def test_refusals(gpu):
         app(k_stride=64), app(k_stride=-128), app(v_stride=130), app(row_type=tk.ROWS_BF16, k_stride=132),
         app(q=x.ptr, q_out=out.ptr), app(k_bias=x.ptr), app(rope_cos=tab), app(rope_sin=tab),
         app(**rope, q=x.ptr), app(**rope, q_out=out.ptr), app(**dict(rope, rope_positions=21)),
+        app(**dict(rope, rope_cos=tab.ptr + 4)), app(**rope, v_bias=x.ptr + 8),
         app(**rope, q=x.ptr, q_out=x.ptr, q_stride=320), app(**rope, q=x.ptr + 4, q_out=out.ptr)]
     for a in bad_append:
         refused(b.append_rows, case.pool, 0, a)
