@@ -22,6 +22,8 @@
 //   O^T += V^T.P^T  the same instruction: P is already in operand order, and
 //                 V's order in the page gives lane (c, h) the same tokens
 // No value crosses lanes until a tile ends.
+#include <type_traits>
+
 #include "attn_common.h"
 #include "e4m3_kernels.h"
 #include "tge_kv.h"
@@ -40,6 +42,9 @@ template <int W>
 struct E4m3Cfg {
   static constexpr int BLOCK = e4m3_block_bytes(W);
   static constexpr int PER_CU = W > 128 ? 1 : W > 64 ? 2 : 3;  // workgroups (= waves per SIMD)
+  // At 256 dims a tile's codes do not fit beside the accumulators: they are
+  // read where they are used, and a wave's own slots refilled by halves (K, V).
+  static constexpr bool LAZY = W > 128;
   static constexpr int TP(int rw) { return rw == 4 ? 4 : 2; }  // pages of a tile
   static constexpr int NB(int rw) { return rw == 1 ? 2 : 4; }  // ring slots of a group
   static constexpr int RING = 16 * BLOCK;                      // (4 / rw) * NB * TP blocks
@@ -110,14 +115,14 @@ __device__ __forceinline__ void store_out4(void* out, long at, int type, float4_
   }
 }
 
-// Copy the page block `n` to LDS at `slot`.
-template <int W, int POLICY>
+// Copy the page block `n` to LDS at `slot`: KiB [FROM, TO) of it.
+template <int W, int POLICY, int FROM, int TO>
 __device__ __forceinline__ void fetch_block(char* slot, const char* blocks, int n, int lane) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int BLOCK = E4m3Cfg<W>::BLOCK;
   const __amdgpu_buffer_rsrc_t rs = make_rsrc(blocks + (size_t)n * BLOCK, BLOCK);
 #pragma unroll
-  for (int i = 0; i < BLOCK / 1024; ++i)
+  for (int i = FROM; i < TO; ++i)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(slot + i * 1024), 16, i * 1024 + lane * 16, 0, 0,
                                              POLICY);
 #endif
@@ -133,17 +138,22 @@ struct E4m3Codes {
   uint32_t v[2][2][NT];  // [block][tokens 4h.. | 8 + 4h..][dims 32i + c]
   uint32_t sa, sb;
 
-  // From the two blocks at `slot`, every read issued before any is waited for.
-  __device__ __forceinline__ void read(const char* slot, const uint32_t* scales, int lane) {
-    constexpr int BLOCK = E4m3Cfg<W>::BLOCK;
-    const int c = lane & 31, h = lane >> 5;
+  __device__ __forceinline__ void read_scales(const uint32_t* scales) {
     const u32x2_t s = *reinterpret_cast<const u32x2_t*>(scales);
-    const char* kp = slot + (c >> 4) * BLOCK + h * 256 + (c & 15) * 16;
+    sa = s[0];
+    sb = s[1];
+  }
+  __device__ __forceinline__ void read_k(const char* slot, int lane) {
+    const int c = lane & 31, h = lane >> 5;
+    const char* kp = slot + (c >> 4) * E4m3Cfg<W>::BLOCK + h * 256 + (c & 15) * 16;
 #pragma unroll
     for (int u = 0; u < KS; ++u) k[u] = *reinterpret_cast<const u32x4_t*>(kp + u * 512);
+  }
+  __device__ __forceinline__ void read_v(const char* slot, int lane) {
+    const int c = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const char* vp = slot + b * BLOCK + 16 * W + (h * 16 + (c & 15)) * 16;
+      const char* vp = slot + b * E4m3Cfg<W>::BLOCK + 16 * W + (h * 16 + (c & 15)) * 16;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if constexpr (W == 64) {
@@ -160,8 +170,6 @@ struct E4m3Codes {
         }
       }
     }
-    sa = s[0];
-    sb = s[1];
   }
 };
 
@@ -171,22 +179,31 @@ struct E4m3Rows {
   static constexpr int KS = E4m3Codes<W>::KS, NT = E4m3Codes<W>::NT;
   half8_t q[KS][2];    // row c, dims 32u + 16h + 8x ..
   f32x16_t o[NT];
-  f32x16_t start;      // -base, sixteen times: the scores' start (0 when they are scaled afterwards)
+  f32x16_t start;      // -base, sixteen times: the scores' start (0 when they are scaled afterwards; not at 256 dims)
   float base, thr, sum;  // of the row; `sum` over the lane's own tokens
   float after;         // factor of the scores once q has entered unscaled, or 0
   int lim;             // the row's last visible position within the item
   int first_lim, last_lim;  // over the wave's rows (wave-uniform)
 
-  __device__ __forceinline__ void set_start() {
+  __device__ __forceinline__ f32x16_t fresh_start() const {
+    f32x16_t s;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) start[r] = after != 0.0f ? 0.0f : -base;
+    for (int r = 0; r < 16; ++r) s[r] = after != 0.0f ? 0.0f : -base;
+    return s;
+  }
+  __device__ __forceinline__ void set_start() {
+    if constexpr (!E4m3Cfg<W>::LAZY) start = fresh_start();
   }
 
-  // Tokens [16 * page, 16 * page + 32).
-  __device__ __forceinline__ void pair(const E4m3Codes<W>& x, int page, int lane) {
+  // Tokens [16 * page, 16 * page + 32): the weights of the lane's tokens to p.
+  __device__ __forceinline__ void scores(const E4m3Codes<W>& x, int page, int lane, half8_t (&p)[2]) {
     const int c = lane & 31, h = lane >> 5;
     const float ks = __uint_as_float((c & 16 ? x.sb : x.sa) << 16);
-    f32x16_t s = start;
+    f32x16_t s;
+    if constexpr (E4m3Cfg<W>::LAZY)
+      s = fresh_start();
+    else
+      s = start;
 #pragma unroll
     for (int u = 0; u < KS; ++u) {
       s = MFMA32x32x16(e4m3x8(x.k[u][0], x.k[u][1], ks), q[u][0], s);
@@ -219,7 +236,6 @@ struct E4m3Rows {
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
       set_start();
     }
-    half8_t p[2];
     const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
@@ -229,6 +245,10 @@ struct E4m3Rows {
       p[r >> 3][r & 7] = w[0];
       p[r >> 3][(r & 7) + 1] = w[1];
     }
+  }
+
+  // The same tokens' values with those weights.
+  __device__ __forceinline__ void values(const E4m3Codes<W>& x, const half8_t (&p)[2]) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float vs = __uint_as_float((b ? x.sb : x.sa) & 0xffff0000u);
@@ -426,7 +446,7 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
 
     // Tile `turn * KS + ks` of the item into its slot (a group past the item's
     // last tile copies that one again).
-    auto fetch = [&](int turn) __attribute__((always_inline)) {
+    auto fetch = [&](int turn, auto from, auto to) __attribute__((always_inline)) {
       char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
       const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
       int n[MINE];
@@ -436,15 +456,18 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
       for (int i = 0; i < MINE; ++i) {
         const int block = __builtin_amdgcn_readfirstlane(n[i]);
         if (it.once)
-          fetch_block<W, kPageLoadPolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
+          fetch_block<W, kPageLoadPolicy, from.value, to.value>(slot + i * C::BLOCK, p.blocks, block, lane);
         else
-          fetch_block<W, kPageReusePolicy>(slot + i * C::BLOCK, p.blocks, block, lane);
+          fetch_block<W, kPageReusePolicy, from.value, to.value>(slot + i * C::BLOCK, p.blocks, block, lane);
       }
     };
+    using First = std::integral_constant<int, 0>;  // (KiB of a block)
+    using Middle = std::integral_constant<int, C::BLOCK / 2048>;
+    using End = std::integral_constant<int, C::BLOCK / 1024>;
     constexpr int AHEAD = RW == 1 ? NB : NB - 1;  // tiles copied before the first is used
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (k < turns) fetch(k);
+      if (k < turns) fetch(k, First{}, End{});
     for (int j = threadIdx.x; j < padded; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
     __syncthreads();  // scales are in LDS
 
@@ -462,21 +485,44 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
           wait_vmcnt<0>();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         const int j = min(j0, padded - TP);
+        const bool seen = j0 < npages && page * 16 <= x.last_lim;
         E4m3Codes<W> codes;
-        codes.read(slot, sh.scales + j, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (turn + NB < turns) fetch(turn + NB);
-        if (j0 < npages && page * 16 <= x.last_lim) x.pair(codes, page, lane);
+        half8_t weights[2];
+        codes.read_scales(sh.scales + j);
+        if constexpr (C::LAZY) {
+          codes.read_k(slot, lane);
+          if (seen) x.scores(codes, page, lane, weights);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (turn + NB < turns) fetch(turn + NB, First{}, Middle{});
+          codes.read_v(slot, lane);
+          if (seen) x.values(codes, weights);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (turn + NB < turns) fetch(turn + NB, Middle{}, End{});
+        } else {
+          codes.read_k(slot, lane);
+          codes.read_v(slot, lane);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (turn + NB < turns) fetch(turn + NB, First{}, End{});
+          if (seen) {
+            x.scores(codes, page, lane, weights);
+            x.values(codes, weights);
+          }
+        }
       } else {
         wait_vmcnt_pages<NB - 2, LOADS>(min(NB - 2, turns - 1 - turn));
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (turn + NB - 1 < turns) fetch(turn + NB - 1);
+        if (turn + NB - 1 < turns) fetch(turn + NB - 1, First{}, End{});
 #pragma unroll
         for (int b = 0; b < TP; b += 2) {
           if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
             E4m3Codes<W> codes;
-            codes.read(slot + b * C::BLOCK, sh.scales + j0 + b, lane);
-            x.pair(codes, page + b, lane);
+            half8_t weights[2];
+            codes.read_scales(sh.scales + j0 + b);
+            codes.read_k(slot + b * C::BLOCK, lane);
+            if constexpr (!C::LAZY) codes.read_v(slot + b * C::BLOCK, lane);
+            x.scores(codes, page + b, lane, weights);
+            if constexpr (C::LAZY) codes.read_v(slot + b * C::BLOCK, lane);
+            x.values(codes, weights);
           }
         }
       }
@@ -508,14 +554,14 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
     sh.base[wr * 32 + c] = top;
     sh.sum[wr * 32 + c] = sum;
   }
-  char* const stage = sh.ring + wave * 32 * W * 4;
+  const int t = thread_here();
+  char* const stage = sh.ring + (t >> 6) * 32 * W * 4;
 #pragma unroll
   for (int i = 0; i < E4m3Rows<W>::NT; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      *reinterpret_cast<float4_t*>(stage + staged<W>(c, 8 * i + 2 * e + h)) =
+      *reinterpret_cast<float4_t*>(stage + staged<W>(t & 31, 8 * i + 2 * e + ((t >> 5) & 1))) =
           float4_t{x.o[i][4 * e], x.o[i][4 * e + 1], x.o[i][4 * e + 2], x.o[i][4 * e + 3]} * f;
-  __syncthreads();
 }
 
 // The staged accumulators of the item's waves become output rows or, for a
@@ -563,9 +609,7 @@ __device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh
 }
 
 template <int W>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(E4m3Cfg<W>::PER_CU, E4m3Cfg<W>::PER_CU)))
-void attention_e4m3_kernel(E4m3Attn p) {
-  __shared__ E4m3Shared<W> sh;
+__device__ __forceinline__ void run_items(const E4m3Attn& p, E4m3Shared<W>& sh) {
   for (int i = blockIdx.x; i >= 0;) {
     const E4m3Item it = load_item(p.items, i);
     i = it.next;
@@ -579,6 +623,24 @@ void attention_e4m3_kernel(E4m3Attn p) {
   }
 }
 
+// (the attributes take numbers only: waves per SIMD)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void attention_e4m3_64(E4m3Attn p) {
+  __shared__ E4m3Shared<64> sh;
+  run_items<64>(p, sh);
+}
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_e4m3_128(E4m3Attn p) {
+  __shared__ E4m3Shared<128> sh;
+  run_items<128>(p, sh);
+}
+// One workgroup fills a compute unit's LDS, so a wave could have 512 registers;
+// but the compiler then keeps the accumulators in the second register file and
+// moves all of them around every pair of pages. With the LDS sized at launch
+// it plans for two waves a SIMD and the 256 registers of the first file.
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_e4m3_256(E4m3Attn p) {
+  extern __shared__ __align__(16) char at_launch[];
+  run_items<256>(p, *reinterpret_cast<E4m3Shared<256>*>(at_launch));
+}
+
 }  // namespace
 
 int e4m3_groups_per_cu(int width) {
@@ -587,11 +649,16 @@ int e4m3_groups_per_cu(int width) {
 
 hipError_t launch_e4m3_attention(int width, int groups, const E4m3Attn& p, hipStream_t stream) {
   if (width == 64)
-    attention_e4m3_kernel<64><<<groups, 256, 0, stream>>>(p);
+    attention_e4m3_64<<<groups, 256, 0, stream>>>(p);
   else if (width == 128)
-    attention_e4m3_kernel<128><<<groups, 256, 0, stream>>>(p);
-  else
-    attention_e4m3_kernel<256><<<groups, 256, 0, stream>>>(p);
+    attention_e4m3_128<<<groups, 256, 0, stream>>>(p);
+  else {
+    constexpr size_t lds = sizeof(E4m3Shared<256>);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attention_e4m3_256),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+    attention_e4m3_256<<<groups, 256, lds, stream>>>(p);
+  }
   return hipGetLastError();
 }
 
