@@ -74,32 +74,59 @@ __device__ __forceinline__ half8_t e4m3x8(uint32_t a, uint32_t b, float scale) {
   return half8_t{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
 
-// Eight q values from element `at` times c, as f16.
-__device__ __forceinline__ half8_t load_q8(const void* q, long at, int type, float c) {
-  float x[8];
+// A lane's q operands: of the row that starts at element `at` the dims 32u +
+// 16h + 8e .., times c, as f16; zero where the lane has no row and past the
+// head's dims. Every load is issued before any is used.
+template <int KS>
+__device__ __forceinline__ void load_q(half8_t (&r)[KS][2], const void* q, long at, int h, int dims, bool live, int type,
+                                       float c) {
+  auto place = [&](int u, int e) __attribute__((always_inline)) {
+    const int d = 32 * u + 16 * h + 8 * e;
+    return at + (d < dims ? d : 0);
+  };
   if (type == TGE_ROWS_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(q) + at);
+    float4_t x[KS][2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (type == TGE_ROWS_BF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const half2_t h = bitcast<half2_t>(w[i]);
-        x[2 * i] = (float)h[0];
-        x[2 * i + 1] = (float)h[1];
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4_t* p = reinterpret_cast<const float4_t*>(static_cast<const float*>(q) + place(u, e));
+        x[u][e][0] = p[0];
+        x[u][e][1] = p[1];
       }
-    }
-  }
-  half8_t r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = (_Float16)(x[i] * c);
-  return r;
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[u][e][i] = (_Float16)(x[u][e][i >> 2][i & 3] * c);
+  } else {
+    u32x4_t w[KS][2];
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        w[u][e] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(q) + place(u, e));
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (type == TGE_ROWS_F16) {  // (c is 1)
+          r[u][e] = bitcast<half8_t>(w[u][e]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            r[u][e][2 * i] = (_Float16)(__uint_as_float(w[u][e][i] << 16) * c);
+            r[u][e][2 * i + 1] = (_Float16)(__uint_as_float(w[u][e][i] & 0xffff0000u) * c);
+          }
+        }
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < KS; ++u)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (!live || 32 * u + 16 * h + 8 * e >= dims) r[u][e] = half8_t{};
 }
 
 // Four outputs, rounded to nearest even for 16-bit rows.
@@ -292,17 +319,16 @@ __device__ __forceinline__ int thread_here() {
   return t;
 }
 
-// The states of a split tile's pieces become its output: the pieces' maxima
-// and sums are read at once and turned into weights in LDS, while the first
-// accumulators are on their way already; every thread adds J chunks of 4 dims,
-// K pieces in flight. The sums are in the pieces' order.
+// The states of a split tile's pieces become its output. Every thread adds J
+// chunks of 4 dims, K pieces in flight, weighted by the pieces' bases, which
+// all threads take from LDS; the sums are in the pieces' order.
 template <int W, int J, int K>
 __device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh, const E4m3Item& it,
                                             const E4m3Merge& m) {
   const auto rs_o = make_rsrc(p.part_o, 0x7fffffff);
   const auto rs_ml = make_rsrc(p.part_ml, 0x7fffffff);
   const int t = thread_here(), rows = m.rows, n = m.n_parts, chunks = rows * (W / 4);
-  float2* const ml = reinterpret_cast<float2*>(sh.ring);  // [n][rows]: (base, sum), then (weight, -)
+  float2* const ml = reinterpret_cast<float2*>(sh.ring);  // [n][rows]: (base, sum)
   const bool fits = (size_t)n * rows * sizeof(float2) <= sizeof(sh.ring);  // else they are read where they are used
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   auto state = [&](int k, int r) __attribute__((always_inline)) {
@@ -325,26 +351,19 @@ __device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh
   load(t, 0);
   // (LDS alone is ordered: the accumulators stay in flight)
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  if (t < rows) {
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) top = fmaxf(top, fits ? ml[k * rows + t].x : state(k, t).x);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float2 v = fits ? ml[k * rows + t] : state(k, t);
-      const float w = v.x == -INFINITY ? 0.0f : pow2i(v.x - top);
-      sum += w * v.y;
-      if (fits) ml[k * rows + t].x = w;
-    }
-    sh.base[t] = top;
-    sh.sum[t] = sum;
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll 1
   for (int i0 = t; i0 < chunks; i0 += 256 * J) {
     float4_t acc[J];
+    float top[J], sum[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) acc[j] = float4_t{0, 0, 0, 0};
+    for (int j = 0; j < J; ++j) {
+      const int r = min(i0 + 256 * j, chunks - 1) / (W / 4);
+      acc[j] = float4_t{0, 0, 0, 0};
+      top[j] = -INFINITY;
+      sum[j] = 0.0f;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) top[j] = fmaxf(top[j], fits ? ml[k * rows + r].x : state(k, r).x);
+    }
 #pragma unroll 1
     for (int k0 = 0; k0 < n; k0 += K) {
       if (i0 != t || k0 != 0) load(i0, k0);
@@ -353,25 +372,20 @@ __device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh
         const int r = min(i0 + 256 * j, chunks - 1) / (W / 4);
 #pragma unroll
         for (int e = 0; e < K; ++e) {
-          float w = 0.0f;
-          if (fits) {
-            w = ml[min(k0 + e, n - 1) * rows + r].x;
-          } else {
-            const float x = state(min(k0 + e, n - 1), r).x;
-            w = x == -INFINITY ? 0.0f : pow2i(x - sh.base[r]);
-          }
-          if (k0 + e < n) acc[j] += o[j][e] * w;
+          const int k = min(k0 + e, n - 1);
+          const float2 v = fits ? ml[k * rows + r] : state(k, r);
+          const float w = k0 + e >= n || v.x == -INFINITY ? 0.0f : pow2i(v.x - top[j]);
+          sum[j] += w * v.y;
+          acc[j] += o[j][e] * w;
         }
       }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int idx = i0 + 256 * j, r = idx / (W / 4), d4 = idx % (W / 4);
-      if (idx < chunks && 4 * d4 < p.dims) {
-        const float sum = sh.sum[r];
+      if (idx < chunks && 4 * d4 < p.dims)
         store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
-                   sum > 0.0f || sum != sum ? div4(acc[j], sum) : float4_t{0, 0, 0, 0});
-      }
+                   sum[j] > 0.0f || sum[j] != sum[j] ? div4(acc[j], sum[j]) : float4_t{0, 0, 0, 0});
     }
   }
   if (t == 0) __hip_atomic_store(p.counters + it.merge, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -411,14 +425,7 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
     x.first_lim = wr * 32 < it.rows ? min(it.ctx + (it.row0 + wr * 32) / p.group, end) : -1;
     x.last_lim = wr * 32 < it.rows ? min(it.ctx + (it.row0 + last) / p.group, end) : -1;
     const long at = (long)(it.q_row + query) * p.q_stride + (long)(it.kv_head * p.group + g - query * p.group) * p.dims;
-#pragma unroll
-    for (int u = 0; u < E4m3Rows<W>::KS; ++u) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = 32 * u + 16 * h + 8 * e;
-        x.q[u][e] = live && d < p.dims ? load_q8(p.q, at + d, p.row_type, factor) : half8_t{};
-      }
-    }
+    load_q(x.q, p.q, at, h, p.dims, live, p.row_type, factor);
     x.base = 0.0f;
     x.thr = -INFINITY;
     x.sum = 0.0f;
@@ -600,9 +607,9 @@ __device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh
     __syncthreads();
     if (sh.flag) {
       if (m.rows * (W / 4) <= 256)
-        merge_parts<W, 1, 16>(p, sh, it, m);
+        merge_parts<W, 1, W == 64 ? 12 : 16>(p, sh, it, m);
       else
-        merge_parts<W, 4, 4>(p, sh, it, m);
+        merge_parts<W, W == 64 ? 2 : 4, W == 64 ? 6 : 4>(p, sh, it, m);
     }
   }
   __syncthreads();  // the shared state is free for the next item

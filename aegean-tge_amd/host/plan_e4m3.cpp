@@ -53,7 +53,7 @@ struct Costs {
 // 431 (379 / 406 / 412), at rw 4 in three, four or five pieces a tile 335 / 313
 // / 327 (349 / 347 / 333). In 256-dim blocks a compute unit holds one workgroup.
 Costs costs_of(int rw, bool prompt, int width, int slots) {
-  if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 4.0, 0.25, 0.05, 8, 32, 1};
+  if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 4.0, 0.25, 0.05, 8, 40, 1};
   const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
   const int grain = rw == 1 ? 8 : 4;
   if (width > 128) return Costs{1.75 * page, 6.0, 6.0 + 4.0 * rw, 1.0, 0.25, grain, 32, 4};
