@@ -451,17 +451,24 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
     }
     __syncthreads();
 
-    // Tile `turn * KS + ks` of the item into its slot (a group past the item's
-    // last tile copies that one again).
-    auto fetch = [&](int turn, auto from, auto to) __attribute__((always_inline)) {
-      char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
-      const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
+    // The blocks of the pages that this wave copies of tile `turn * KS + ks` (a
+    // group past the item's last tile copies that one again), and their copies
+    // into the tile's slot.
+    struct Blocks {
       int n[MINE];
+    };
+    auto blocks_of = [&](int turn) __attribute__((always_inline)) {
+      const int j0 = min(turn * KS + ks, ntiles - 1) * TP + wr * MINE;
+      Blocks b;
 #pragma unroll
-      for (int i = 0; i < MINE; ++i) n[i] = sh.ids[j0 + i];
+      for (int i = 0; i < MINE; ++i) b.n[i] = sh.ids[j0 + i];
+      return b;
+    };
+    auto fetch = [&](int turn, const Blocks& b, auto from, auto to) __attribute__((always_inline)) {
+      char* const slot = ring + (turn % NB) * TP * C::BLOCK + wr * MINE * C::BLOCK;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
-        const int block = __builtin_amdgcn_readfirstlane(n[i]);
+        const int block = __builtin_amdgcn_readfirstlane(b.n[i]);
         if (it.once)
           fetch_block<W, kPageLoadPolicy, from.value, to.value>(slot + i * C::BLOCK, p.blocks, block, lane);
         else
@@ -474,7 +481,7 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
     constexpr int AHEAD = RW == 1 ? NB : NB - 1;  // tiles copied before the first is used
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (k < turns) fetch(k, First{}, End{});
+      if (k < turns) fetch(k, blocks_of(k), First{}, End{});
     for (int j = threadIdx.x; j < padded; j += 256) sh.scales[j] = p.scales[sh.ids[j]];
     __syncthreads();  // scales are in LDS
 
@@ -496,29 +503,31 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
         E4m3Codes<W> codes;
         half8_t weights[2];
         codes.read_scales(sh.scales + j);
+        const Blocks next = blocks_of(turn + NB);
         if constexpr (C::LAZY) {
           codes.read_k(slot, lane);
           if (seen) x.scores(codes, page, lane, weights);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (turn + NB < turns) fetch(turn + NB, First{}, Middle{});
+          if (turn + NB < turns) fetch(turn + NB, next, First{}, Middle{});
           codes.read_v(slot, lane);
           if (seen) x.values(codes, weights);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (turn + NB < turns) fetch(turn + NB, Middle{}, End{});
+          if (turn + NB < turns) fetch(turn + NB, next, Middle{}, End{});
         } else {
           codes.read_k(slot, lane);
           codes.read_v(slot, lane);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (turn + NB < turns) fetch(turn + NB, First{}, End{});
+          if (turn + NB < turns) fetch(turn + NB, next, First{}, End{});
           if (seen) {
             x.scores(codes, page, lane, weights);
             x.values(codes, weights);
           }
         }
       } else {
+        const Blocks next = blocks_of(turn + NB - 1);
         wait_vmcnt_pages<NB - 2, LOADS>(min(NB - 2, turns - 1 - turn));
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (turn + NB - 1 < turns) fetch(turn + NB - 1, First{}, End{});
+        if (turn + NB - 1 < turns) fetch(turn + NB - 1, next, First{}, End{});
 #pragma unroll
         for (int b = 0; b < TP; b += 2) {
           if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
