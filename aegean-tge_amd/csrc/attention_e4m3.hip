@@ -274,14 +274,35 @@ struct E4m3Rows {
     }
   }
 
+  __device__ __forceinline__ void pair(const E4m3Codes<W>& x, int page, int lane) {
+    half8_t p[2];
+    scores(x, page, lane, p);
+    values(x, p);
+  }
+
   // The same tokens' values with those weights.
   __device__ __forceinline__ void values(const E4m3Codes<W>& x, const half8_t (&p)[2]) {
+#ifdef E4_V2
+    half8_t v[2];
+    v[0] = e4m3x8(x.v[0][0][0], x.v[0][1][0], __uint_as_float(x.sa & 0xffff0000u));
+#pragma unroll
+    for (int k = 0; k < 2 * NT; ++k) {
+      const int b = k / NT, i = k % NT;
+      if (k + 1 < 2 * NT) {
+        const int b1 = (k + 1) / NT, i1 = (k + 1) % NT;
+        v[(k + 1) & 1] = e4m3x8(x.v[b1][0][i1], x.v[b1][1][i1], __uint_as_float((b1 ? x.sb : x.sa) & 0xffff0000u));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      o[i] = MFMA32x32x16(v[k & 1], p[b], o[i]);
+    }
+#else
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float vs = __uint_as_float((b ? x.sb : x.sa) & 0xffff0000u);
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] = MFMA32x32x16(e4m3x8(x.v[b][0][i], x.v[b][1][i], vs), p[b], o[i]);
     }
+#endif
   }
 };
 
@@ -518,10 +539,7 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
           codes.read_v(slot, lane);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           if (turn + NB < turns) fetch(turn + NB, next, First{}, End{});
-          if (seen) {
-            x.scores(codes, page, lane, weights);
-            x.values(codes, weights);
-          }
+          if (seen) x.pair(codes, page, lane);
         }
       } else {
         const Blocks next = blocks_of(turn + NB - 1);
@@ -532,13 +550,17 @@ __device__ __forceinline__ void run_item(const E4m3Attn& p, E4m3Shared<W>& sh, c
         for (int b = 0; b < TP; b += 2) {
           if (j0 + b < npages && (page + b) * 16 <= x.last_lim) {
             E4m3Codes<W> codes;
-            half8_t weights[2];
             codes.read_scales(sh.scales + j0 + b);
             codes.read_k(slot + b * C::BLOCK, lane);
-            if constexpr (!C::LAZY) codes.read_v(slot + b * C::BLOCK, lane);
-            x.scores(codes, page + b, lane, weights);
-            if constexpr (C::LAZY) codes.read_v(slot + b * C::BLOCK, lane);
-            x.values(codes, weights);
+            if constexpr (C::LAZY) {
+              half8_t weights[2];
+              x.scores(codes, page + b, lane, weights);
+              codes.read_v(slot + b * C::BLOCK, lane);
+              x.values(codes, weights);
+            } else {
+              codes.read_v(slot + b * C::BLOCK, lane);
+              x.pair(codes, page + b, lane);
+            }
           }
         }
       }

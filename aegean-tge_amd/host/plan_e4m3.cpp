@@ -27,7 +27,8 @@ using Group = std::vector<Piece>;
 struct Costs {
   double page;    // a page
   double start;   // an item's start and end
-  double merge;   // a tile that is cut: its merge
+  double cut;     // a piece of a cut tile: its partial state and share of the merge
+  double merge;   // a launch with cut tiles: the last merge
   double solo;    // cost of a page, relative, where the compute unit's other slots are idle
   double uneven;  // what the longest item adds to a launch, relative
   int grain;      // pages that the waves share out at a time
@@ -53,11 +54,11 @@ struct Costs {
 // 431 (379 / 406 / 412), at rw 4 in three, four or five pieces a tile 335 / 313
 // / 327 (349 / 347 / 333). In 256-dim blocks a compute unit holds one workgroup.
 Costs costs_of(int rw, bool prompt, int width, int slots) {
-  if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 4.0, 0.25, 0.05, 8, 40, 1};
+  if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 2.0, 4.0, 0.25, 0.05, 8, 40, 1};
   const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
   const int grain = rw == 1 ? 8 : 4;
-  if (width > 128) return Costs{1.75 * page, 6.0, 6.0 + 4.0 * rw, 1.0, 0.25, grain, 32, 4};
-  return Costs{page * width / 128.0, 4.0, 6.0 + 2.0 * rw, 0.7, 0.25, grain, 32, 4};
+  if (width > 128) return Costs{1.75 * page, 6.0, 6.0 * rw, 6.0 + 2.0 * rw, 1.0, 0.25, grain, 32, 4};
+  return Costs{page * width / 128.0, 4.0, 3.0 * rw, 4.0 + rw, 0.7, 0.25, grain, 32, 4};
 }
 
 // Each tile in equal pieces of at most `len` pages, a piece a group.
@@ -83,7 +84,7 @@ int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, doub
     for (const Tile& t : tiles) {
       const int of = ceil_div(t.pages, len);
       n += of;
-      total += t.pages * c.page + of * c.start;
+      total += t.pages * c.page + of * c.start + (of > 1 ? of * c.cut : 0.0);
     }
     if (best && n > (long long)slots * c.rounds) break;
     const double t = c.time(total, n, std::min(len, most), slots, len < most);
