@@ -282,27 +282,12 @@ struct E4m3Rows {
 
   // The same tokens' values with those weights.
   __device__ __forceinline__ void values(const E4m3Codes<W>& x, const half8_t (&p)[2]) {
-#ifdef E4_V2
-    half8_t v[2];
-    v[0] = e4m3x8(x.v[0][0][0], x.v[0][1][0], __uint_as_float(x.sa & 0xffff0000u));
-#pragma unroll
-    for (int k = 0; k < 2 * NT; ++k) {
-      const int b = k / NT, i = k % NT;
-      if (k + 1 < 2 * NT) {
-        const int b1 = (k + 1) / NT, i1 = (k + 1) % NT;
-        v[(k + 1) & 1] = e4m3x8(x.v[b1][0][i1], x.v[b1][1][i1], __uint_as_float((b1 ? x.sb : x.sa) & 0xffff0000u));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      o[i] = MFMA32x32x16(v[k & 1], p[b], o[i]);
-    }
-#else
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float vs = __uint_as_float((b ? x.sb : x.sa) & 0xffff0000u);
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] = MFMA32x32x16(e4m3x8(x.v[b][0][i], x.v[b][1][i], vs), p[b], o[i]);
     }
-#endif
   }
 };
 

@@ -51,8 +51,8 @@ struct Costs {
 // rw) pay less for the copies. Fitted at 28/4 heads of 128 dims, rw 1 / 2 / 4,
 // us measured (by this model): 2048 tokens 61 / 52 / 51 (59 / 53 / 53), 512
 // behind 1536 25 / 32 / 47 (25 / 31 / 53), 1333 behind 14003 uncut 363 / 388 /
-// 431 (379 / 406 / 412), at rw 4 in three, four or five pieces a tile 335 / 313
-// / 327 (349 / 347 / 333). In 256-dim blocks a compute unit holds one workgroup.
+// 431 (379 / 406 / 412). A cut piece: 4096 tokens at rw 4 uncut 140 us, in halves
+// 162; at rw 2 144 and 168. In 256-dim blocks a compute unit holds one workgroup.
 Costs costs_of(int rw, bool prompt, int width, int slots) {
   if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 2.0, 4.0, 0.25, 0.05, 8, 40, 1};
   const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
