@@ -169,6 +169,14 @@ def attend(cache, ctx, q, qh, scale=None):
     return out.reshape(n, -1), bound.reshape(n, -1)
 
 
+# Steps whose attention items read more pages than the kernel holds block
+# numbers for at a time (1024): (query heads, KV heads, head_dim, ctx, new
+# tokens, sessions over the same pages) -> rows of a tile / 32.
+LONG_ITEMS = {(4, 1, 64, 17000, 1, 900): 1, (40, 1, 128, 17000, 1, 600): 2, (8, 1, 256, 17000, 1, 300): 1,
+              (64, 1, 256, 17000, 1, 300): 2, (64, 1, 64, 17000, 2000, 1): 4, (128, 1, 128, 17000, 1100, 1): 2,
+              (128, 1, 128, 17000, 2300, 1): 4}
+
+
 class Rows:
     """Device rows of a type, `gap` elements between them, the gaps (and the
     rows behind the last) filled with a pattern that must stay."""

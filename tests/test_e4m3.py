@@ -4,6 +4,9 @@ import pytest
 
 import _e4m3 as M
 import tge_kv as tk
+from test_host_plan import build_and_run
+
+PLAN_CHECK = ["aegean-tge_amd/host/plan.cpp", "aegean-tge_amd/host/plan_e4m3.cpp", "tests/native/plan_e4m3_check.cpp"]
 
 
 def test_model_codec():
@@ -53,3 +56,15 @@ def test_calls_refuse_null(tk):
     assert L.tge_kv_append_rows(None, None, 0, None, None) == tk.ERR_INVALID
     assert L.tge_attention_rows(None, None, 0, None, None) == tk.ERR_INVALID
     assert L.tge_qwen2_kv_layer_rows(None, 0, None, None, None) == tk.ERR_INVALID
+
+
+def test_plans_under_sanitizers(tmp_path):
+    assert "plan_e4m3_check ok" in build_and_run(tmp_path, "plan_e4m3_check", PLAN_CHECK)
+
+
+def test_plans_of_the_long_items(tmp_path):
+    """The GPU tests' long items are what they are named for."""
+    out = build_and_run(tmp_path, "plan_e4m3_check", PLAN_CHECK, M.LONG_ITEMS)
+    for (case, rw), line in zip(M.LONG_ITEMS.items(), out.splitlines(), strict=True):
+        p = dict(zip(line.split()[::2], map(int, line.split()[1::2])))
+        assert p["longest"] > 1024 and p["rw"] == rw, (case, line)

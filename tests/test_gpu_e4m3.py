@@ -243,6 +243,25 @@ def test_prompt_large(gpu, qh, kvh, hd, ctx, n):
     sampled(case, tk.ROWS_BF16, 37)
 
 
+@pytest.mark.parametrize("qh,kvh,hd,ctx,n,sessions", M.LONG_ITEMS)
+def test_long_items(gpu, qh, kvh, hd, ctx, n, sessions):
+    """Items of more pages than the block numbers held at a time, many
+    sessions over one session's pages (some rows checked)."""
+    case = one_session(qh, kvh, hd, ctx, n, seed=35)
+    case.fill(tk.ROWS_BF16)
+    append(case, case.step_rows(tk.ROWS_BF16), tk.ROWS_BF16)
+    rows = n * sessions
+    q = M.as_type(case.rng.standard_normal((rows, qh * hd)), tk.ROWS_BF16)
+    dq, out = M.Rows(q, tk.ROWS_BF16), M.Rows(np.zeros_like(q), tk.ROWS_BF16)
+    b = case.plan([tk.Session(ctx, n, case.pages[0])] * sessions)
+    b.attention_rows(case.pool, 0, tk.attention_rows_args(tk.ROWS_BF16, dq, out))
+    tk.hip().sync()
+    got = out.read()
+    for i in (0, rows // 2, rows - 1):
+        want, bound = M.attend(case.cache[0], ctx + i % n, q[i: i + 1], qh)
+        check(got[i: i + 1], want, bound, tk.ROWS_BF16)
+
+
 @pytest.mark.parametrize("qh,kvh,hd", [(28, 4, 128), (16, 8, 256), (14, 2, 64)])
 def test_mixed(gpu, qh, kvh, hd):
     case = M.Case(qh, kvh, hd, [(300, 1), (40, 70), (0, 3), (513, 4), (7, 100)], seed=11)
@@ -375,6 +394,40 @@ def test_driver_serves_16_bit_rows(gpu):
             q = M.as_type(M.rotate(q, np.zeros(qh * hd), cos[pos], sin[pos], hd), t)
             assert np.array_equal(rot.read(), q)
             check(out.read(), *M.attend(cache, start, q, qh), t)
+    m.close()
+
+
+def test_driver_shares_and_copies_pages(gpu):
+    """A sequence takes over 47 of another's 50 tokens and writes its own behind
+    them: the page that both hold is copied, codes and scales, and neither sees
+    the other's rows afterwards."""
+    qh, kvh, hd, t = 8, 2, 128, tk.ROWS_BF16
+    m = tk.Qwen2KvPath(1, qh, kvh, hd, context=256, sequences=2, pages=40, fmt=tk.KV_E4M3)
+    rng = np.random.default_rng(37)
+    caches = [M.Cache(kvh, hd), M.Cache(kvh, hd)]
+
+    def step(seq, start, n):
+        if n == 1:
+            m.begin_forward(seq, start)
+        else:
+            m.begin_prefill(seq, start, n)
+        q, k, v = (M.as_type(rng.standard_normal((n, h * hd)) * (1 + start), t) for h in (qh, kvh, kvh))
+        rows = [M.Rows(x, t) for x in (q / np.float32(1 + start), k, v)]
+        out = M.Rows(np.zeros((n, qh * hd)), t)
+        m.layer_rows(0, tk.append_rows_args(t, *rows[1:]), tk.attention_rows_args(t, rows[0], out))
+        tk.hip().sync()
+        caches[seq].append(start, k, v)
+        check(out.read(), *M.attend(caches[seq], start, rows[0].read(), qh), t)
+
+    tokens = list(range(100, 150))
+    step(0, 0, 50)
+    assert m.remember_prefix(0, tokens) == 50
+    assert m.attach_prefix(1, tokens[:47] + [5] * 20) == 47
+    caches[1].codes = [c[:47].copy() for c in caches[0].codes]
+    caches[1].exps = [e[:3].copy() for e in caches[0].exps]
+    step(1, 47, 20)  # (louder rows: the copy's scales and older codes change)
+    step(0, 50, 1)
+    step(1, 67, 1)
     m.close()
 
 
