@@ -12,6 +12,7 @@
 #include <functional>
 #include <mutex>
 #include <stdexcept>
+#include <new>
 #include <string>
 #include <array>
 #include <vector>
@@ -537,7 +538,11 @@ int plan_e4m3(tge_batch* b, hipStream_t hs) {
                 "batch_plan: the stream is capturing (the plan is uploaded from host memory, which a "
                 "graph would replay stale; plan first, then capture the calls)");
   E4m3Plan& e = b->e4;
-  tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
+  try {
+    tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
+  } catch (const std::bad_alloc&) {
+    return fail(TGE_ERR_CAPACITY, "batch_plan: out of host memory");
+  }
   const auto& L = e.lists;
   if ((size_t)L.parts * L.part_rows * st.block_dims * sizeof(float) > 0x7fffffffu)
     return fail(TGE_ERR_CAPACITY, "batch_plan: the step's partial states exceed 2 GiB");

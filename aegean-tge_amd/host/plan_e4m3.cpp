@@ -75,16 +75,20 @@ std::vector<Group> pieces(const std::vector<Tile>& tiles, int len, const Costs& 
 
 // Of the piece lengths the one with the least time.
 int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, double* time) {
+  // (tiles of one length count together)
   int most = 0, best = 0;
   for (const Tile& t : tiles) most = std::max(most, t.pages);
+  std::vector<int> count((std::size_t)most + 1, 0), lengths;
+  for (const Tile& t : tiles)
+    if (count[(std::size_t)t.pages]++ == 0) lengths.push_back(t.pages);
   *time = 1e30;
   for (int len = ceil_div(most, c.grain) * c.grain;;) {
     long long n = 0;
     double total = 0.0;
-    for (const Tile& t : tiles) {
-      const int of = ceil_div(t.pages, len);
-      n += of;
-      total += t.pages * c.page + of * c.start + (of > 1 ? of * c.cut : 0.0);
+    for (int pages : lengths) {
+      const int of = ceil_div(pages, len), k = count[(std::size_t)pages];
+      n += (long long)of * k;
+      total += k * (pages * c.page + of * c.start + (of > 1 ? of * c.cut : 0.0));
     }
     if (best && n > (long long)slots * c.rounds) break;
     const double t = c.time(total, n, std::min(len, most), slots, len < most);
@@ -103,43 +107,68 @@ int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, doub
 // launch end after 65 and 80 us, two workgroups a unit), so the share of the
 // k-th of `per_cu` is smaller by `kLater` for each one before it.
 constexpr double kLater = 0.18;
-std::vector<Group> shares(const std::vector<Tile>& tiles, int slots, int per_cu, const Costs& c, double* time) {
-  double total = 0.0;
-  for (const Tile& t : tiles) total += t.pages * c.page + c.start;
-  const int least = std::min(c.least, 2 * c.grain), cus = std::max(1, slots / per_cu);
-  const double middle = 1.0 - kLater * (per_cu - 1) / 2;
-  double share = std::max(total / slots + 0.5 * c.start, c.least * c.page + c.start);
-  std::vector<Group> groups;
-  bool cut = false;
-  for (;; share *= 1.01) {  // (until the shares are no more than the slots)
-    groups.clear();
-    cut = false;
-    double left = 0.0;
-    for (std::size_t i = 0; i < tiles.size(); ++i) {
-      const int pages = tiles[i].pages;
-      std::vector<std::pair<int, int>> at;  // (end page, group) of each piece
-      for (int begin = 0; begin < pages;) {
-        if (left < c.start + least * c.page || groups.empty()) {
-          const int later = std::min((int)groups.size() / cus, per_cu - 1);
-          left = share * (1.0 - kLater * later) / middle;
-          groups.emplace_back();
-        }
-        int n = std::min(pages - begin, std::max(least, (int)((left - c.start) / c.page) / c.grain * c.grain));
-        if (pages - begin - n < least) n = pages - begin;  // (no slivers)
-        begin += n;
-        left -= n * c.page + c.start;
-        at.emplace_back(begin, (int)groups.size() - 1);
-      }
-      cut = cut || at.size() > 1;
-      for (std::size_t k = 0; k < at.size(); ++k)
-        groups[(std::size_t)at[k].second].push_back(
-            Piece{(int)i, k ? at[k - 1].first : 0, at[k].first, (int)k, (int)at.size()});
-    }
-    if ((int)groups.size() <= slots) break;
+class Shares {
+ public:
+  Shares(const std::vector<Tile>& tiles, int slots, int per_cu, const Costs& c)
+      : tiles_(tiles), per_cu_(per_cu), cus_(std::max(1, slots / per_cu)), c_(c) {
+    double total = 0.0;
+    for (const Tile& t : tiles) total += t.pages * c.page + c.start;
+    share_ = std::max(total / slots + 0.5 * c.start, c.least * c.page + c.start);
+    bool cut = false;
+    auto count = [&](int group, const Tile& t, int begin, int end) {
+      cut = cut || begin > 0 || end < t.pages;
+      return group < slots;
+    };
+    while (!walk(count)) share_ *= 1.01;  // (until the shares are no more than the slots)
+    time = share_ + 0.5 * c.start + (cut ? c.merge : 0.0);
   }
-  *time = share + 0.5 * c.start + (cut ? c.merge : 0.0);
-  return groups;
-}
+
+  std::vector<Group> groups() const {
+    std::vector<Group> out;
+    std::size_t first = 0;  // group of the tile's first piece
+    walk([&](int group, const Tile& t, int begin, int end) {
+      if (out.size() <= (std::size_t)group) out.emplace_back();
+      if (begin == 0) first = (std::size_t)group;
+      const int tile = (int)(&t - tiles_.data());
+      out.back().push_back(Piece{tile, begin, end, group - (int)first, 1});
+      if (end == t.pages)  // a group holds one piece of a tile at most
+        for (std::size_t g = first; g < out.size(); ++g)
+          (g == first ? out[g].back() : out[g].front()).of = group - (int)first + 1;
+      return true;
+    });
+    return out;
+  }
+
+  double time = 0.0;
+
+ private:
+  // put(group, tile, begin, end) for every piece, until it returns false.
+  template <class Put>
+  bool walk(Put put) const {
+    const int least = std::min(c_.least, 2 * c_.grain);
+    const double middle = 1.0 - kLater * (per_cu_ - 1) / 2;
+    double left = 0.0;
+    int group = -1;
+    for (const Tile& t : tiles_)
+      for (int begin = 0; begin < t.pages;) {
+        if (left < c_.start + least * c_.page || group < 0) {
+          ++group;
+          left = share_ * (1.0 - kLater * std::min(group / cus_, per_cu_ - 1)) / middle;
+        }
+        int n = std::min(t.pages - begin, std::max(least, (int)((left - c_.start) / c_.page) / c_.grain * c_.grain));
+        if (t.pages - begin - n < least) n = t.pages - begin;  // (no slivers)
+        if (!put(group, t, begin, begin + n)) return false;
+        begin += n;
+        left -= n * c_.page + c_.start;
+      }
+    return true;
+  }
+
+  const std::vector<Tile>& tiles_;
+  int per_cu_, cus_;
+  Costs c_;
+  double share_ = 0.0;
+};
 
 // Workgroup b runs on XCD b mod 8, each with an L2 of its own and slots / 8
 // workgroups: the pieces of one (session, KV head), which read the same pages,
@@ -246,12 +275,12 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
     return t;
   };
 
-  std::vector<std::vector<E4m3Item>> all;
+  // A workgroup's first item has its index, its later ones follow the firsts.
   auto add = [&](const std::vector<Tile>& tiles, const std::vector<Group>& groups, bool once) {
     // pieces of a cut tile own consecutive partial slots
     std::vector<int> merge(tiles.size(), -1);
     for (const Group& gr : groups) {
-      all.emplace_back();
+      std::size_t at = (std::size_t)out.groups++;
       for (const Piece& p : gr) {
         const Tile& t = tiles[(std::size_t)p.tile];
         const SessionRec& r = s.sessions[(std::size_t)t.session];
@@ -263,8 +292,13 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
           out.parts += p.of;
         }
         const int part = p.of > 1 ? out.merges[(std::size_t)m].first_part + p.index : -1;
-        all.back().push_back(E4m3Item{t.kv_head, p.begin, p.end, part, t.row0, t.rows, r.ctx, r.q_row, r.table_off, m,
-                                      t.rw, once ? 1 : 0, -1, {}});
+        if (&p != &gr[0]) {
+          out.items[at].next = (int)out.items.size();
+          at = out.items.size();
+          out.items.emplace_back();
+        }
+        out.items[at] = E4m3Item{t.kv_head, p.begin, p.end, part, t.row0, t.rows, r.ctx, r.q_row, r.table_off, m,
+                                 t.rw, once ? 1 : 0, -1, {}};
       }
     }
   };
@@ -272,11 +306,11 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
   double time = 0.0;
   auto plan_decode = [&](int n, double* t) {
     const Costs c = costs_of(1, false, s.block_dims, slots);
-    double a = 0.0, b = 0.0;
-    const int len = piece_length(decode, n, c, &a);
-    std::vector<Group> y = shares(decode, n, per_cu, c, &b);
-    *t = std::min(a, b);
-    return a <= b ? pieces(decode, len, c) : y;
+    const int len = piece_length(decode, n, c, t);
+    const Shares x(decode, n, per_cu, c);
+    if (*t <= x.time) return pieces(decode, len, c);
+    *t = x.time;
+    return x.groups();
   };
   auto plan_prompts = [&](int n, std::vector<Tile>* tiles, double* t) {
     std::vector<Group> best;
@@ -310,22 +344,9 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
     dg = plan_decode(n, &d);
     pg = plan_prompts(slots - n, &pt, &p);
   }
+  out.items.resize(dg.size() + pg.size());
   add(decode, dg, true);
   add(pt, pg, false);
-  // A workgroup's first item has its index, its later ones follow the firsts.
-  out.groups = (int)all.size();
-  out.items.resize(all.size());
-  for (std::size_t i = 0; i < all.size(); ++i) {
-    std::size_t at = i;
-    for (std::size_t k = 0; k < all[i].size(); ++k) {
-      if (k) {
-        out.items[at].next = (int)out.items.size();
-        at = out.items.size();
-        out.items.emplace_back();
-      }
-      out.items[at] = all[i][k];
-    }
-  }
 }
 
 }  // namespace tge::plan

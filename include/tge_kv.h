@@ -352,9 +352,10 @@ int tge_batch_attention(const tge_batch* batch, const tge_kv_pool* pool,
  * The two calls below take rows of fp32, f16 or bf16 with a stride, such as
  * slices of one projection's output: `*_stride` elements lie between rows (0:
  * none lie between them). Bases (rotary tables and biases too) are 16-byte
- * aligned and strides multiples of 16 bytes. The fp32 calls on such a pool (tge_kv_append, tge_kv_append_rope,
- * tge_decode_attention, tge_decode_step, tge_prefill_attention,
- * tge_batch_attention, the driver) are the same kernels with fp32 rows.
+ * aligned and strides multiples of 16 bytes. The fp32 calls on such a pool
+ * (tge_kv_append, tge_kv_append_rope, tge_decode_attention, tge_decode_step,
+ * tge_prefill_attention, tge_batch_attention, the driver) are the same kernels
+ * with fp32 rows.
  * tge_decode_attention_static, tge_attention_group and a static sparse subset
  * are refused on such a pool (TGE_ERR_INVALID), and so are these two calls on
  * any other pool, on a pool of another device than the current one, and
@@ -410,9 +411,11 @@ typedef struct {
 
 /* Attention of every new token of the batch over its session's positions 0 ..
  * its own, any mix of decoding, verifying and prompt sessions in one launch.
- * q is scaled and rounded to f16 once, softmax weights are f16, sums and
- * accumulators fp32, out is rounded once. A row of NaN gives NaN and touches no
- * other row. The same inputs give the same bits on every run. */
+ * q is scaled and rounded to f16 once (rows of f16 enter as they are, the
+ * scores are scaled; a scaled value past f16's largest, 65504, counts as
+ * infinite), softmax weights are f16, sums and accumulators fp32, out is
+ * rounded once. A row of NaN gives NaN and touches no other row. The same
+ * inputs give the same bits on every run. */
 int tge_attention_rows(const tge_batch* batch, const tge_kv_pool* pool, int layer,
                        const tge_attention_rows_args* args, void* stream);
 
