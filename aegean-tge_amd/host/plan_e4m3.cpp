@@ -55,10 +55,10 @@ struct Costs {
 // 162; at rw 2 144 and 168. In 256-dim blocks a compute unit holds one workgroup.
 Costs costs_of(int rw, bool prompt, int width, int slots) {
   if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 2.0, 4.0, 0.25, 0.05, 8, 40, 1};
-  const double page = rw == 1 ? 0.16 : rw == 2 ? 0.30 : 0.544;
+  const double page = rw == 1 ? 0.155 : rw == 2 ? 0.285 : 0.53;
   const int grain = rw == 1 ? 8 : 4;
-  if (width > 128) return Costs{1.75 * page, 6.0, 6.0 * rw, 6.0 + 2.0 * rw, 1.0, 0.25, grain, 32, 4};
-  return Costs{page * width / 128.0, 4.0, 3.0 * rw, 4.0 + rw, 0.7, 0.25, grain, 32, 4};
+  if (width > 128) return Costs{1.05 * page, 6.0, 6.0 * rw, 6.0 + 2.0 * rw, 1.0, 0.25, grain, 32, 4};
+  return Costs{width < 128 ? 0.66 * page : page, 4.0, 3.0 * rw, 4.0 + rw, 0.7, 0.25, grain, 32, 4};
 }
 
 // Each tile in equal pieces of at most `len` pages, a piece a group.
@@ -114,13 +114,15 @@ class Shares {
     double total = 0.0;
     for (const Tile& t : tiles) total += t.pages * c.page + c.start;
     share_ = std::max(total / slots + 0.5 * c.start, c.least * c.page + c.start);
-    bool cut = false;
     auto count = [&](int group, const Tile& t, int begin, int end) {
-      cut = cut || begin > 0 || end < t.pages;
+      cut_pieces += begin > 0 || end < t.pages;
       return group < slots;
     };
-    while (!walk(count)) share_ *= 1.01;  // (until the shares are no more than the slots)
-    time = share_ + 0.5 * c.start + (cut ? c.merge : 0.0);
+    while (!walk(count)) {  // (until the shares are no more than the slots)
+      share_ *= 1.01;
+      cut_pieces = 0;
+    }
+    time = share_ + 0.5 * c.start + (cut_pieces ? c.merge : 0.0);
   }
 
   std::vector<Group> groups() const {
@@ -139,7 +141,8 @@ class Shares {
     return out;
   }
 
-  double time = 0.0;
+  double time = 0.0;  // (without the cut pieces' own)
+  int cut_pieces = 0;
 
  private:
   // put(group, tile, begin, end) for every piece, until it returns false.
@@ -317,6 +320,11 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
     *t = 1e30;
     for (int rw : {4, 2, 1}) {
       std::vector<Tile> x = prompt_tiles(rw);
+      int shortest = x[0].pages, longest = 0;
+      for (const Tile& i : x) {
+        shortest = std::min(shortest, i.pages);
+        longest = std::max(longest, i.pages);
+      }
       if (rw < 4 && best.size() >= 4 * (std::size_t)n) break;  // (large tiles alone fill the device)
       const Costs c = costs_of(rw, true, s.block_dims, slots);
       double e = 0.0;
@@ -324,6 +332,19 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
       if (e < *t) {
         *t = e;
         best = pieces(x, len, c);
+        *tiles = x;
+      }
+      // Tiles of like length, too few to even out over the slots, as shares
+      // (pieces / shares, us: 28/4 heads of 128 dims, 1333 behind 14003 317 /
+      // 300, 1000 behind 30000 462 / 440; 16/8 of 256, 2000 behind 30000 1100 /
+      // 1058; not 28/4 of 128, 4096 tokens 139 / 225, 2048 behind 2048 104 /
+      // 130, whose tiles' lengths differ; nor 64/8, 2048 behind 8000 572 / 606,
+      // two tiles a slot).
+      if (2 * shortest < longest || x.size() >= 2 * (std::size_t)n) continue;
+      const Shares y(x, n, 1, c);
+      if (y.time + c.cut * y.cut_pieces / n < *t) {
+        *t = y.time + c.cut * y.cut_pieces / n;
+        best = y.groups();
         *tiles = std::move(x);
       }
     }
