@@ -102,15 +102,14 @@ int piece_length(const std::vector<Tile>& tiles, int slots, const Costs& c, doub
   return best;
 }
 
-// The tiles end to end, cut into shares, a share a group. Workgroups that land
-// on a compute unit after others get less of it (equal shares of a decode
-// launch end after 65 and 80 us, two workgroups a unit), so the share of the
-// k-th of `per_cu` is smaller by `kLater` for each one before it.
-constexpr double kLater = 0.18;
+// The tiles end to end, cut into equal shares, a share a group. (Smaller shares
+// for the workgroups that land on a compute unit after others, or a part of
+// every tile in a queue for those that end first, gained nothing: 64 sessions
+// of 1k to 32k tokens, 28/4 heads of 128 dims, 118.8 us; 121.8 with shares 18 %
+// apart, 121 with a tenth of the pages queued, 127 with a fifth.)
 class Shares {
  public:
-  Shares(const std::vector<Tile>& tiles, int slots, int per_cu, const Costs& c)
-      : tiles_(tiles), per_cu_(per_cu), cus_(std::max(1, slots / per_cu)), c_(c) {
+  Shares(const std::vector<Tile>& tiles, int slots, const Costs& c) : tiles_(tiles), c_(c) {
     double total = 0.0;
     for (const Tile& t : tiles) total += t.pages * c.page + c.start;
     share_ = std::max(total / slots + 0.5 * c.start, c.least * c.page + c.start);
@@ -149,14 +148,13 @@ class Shares {
   template <class Put>
   bool walk(Put put) const {
     const int least = std::min(c_.least, 2 * c_.grain);
-    const double middle = 1.0 - kLater * (per_cu_ - 1) / 2;
     double left = 0.0;
     int group = -1;
     for (const Tile& t : tiles_)
       for (int begin = 0; begin < t.pages;) {
         if (left < c_.start + least * c_.page || group < 0) {
           ++group;
-          left = share_ * (1.0 - kLater * std::min(group / cus_, per_cu_ - 1)) / middle;
+          left = share_;
         }
         int n = std::min(t.pages - begin, std::max(least, (int)((left - c_.start) / c_.page) / c_.grain * c_.grain));
         if (t.pages - begin - n < least) n = t.pages - begin;  // (no slivers)
@@ -168,7 +166,6 @@ class Shares {
   }
 
   const std::vector<Tile>& tiles_;
-  int per_cu_, cus_;
   Costs c_;
   double share_ = 0.0;
 };
@@ -310,7 +307,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
   auto plan_decode = [&](int n, double* t) {
     const Costs c = costs_of(1, false, s.block_dims, slots);
     const int len = piece_length(decode, n, c, t);
-    const Shares x(decode, n, per_cu, c);
+    const Shares x(decode, n, c);
     if (*t <= x.time) return pieces(decode, len, c);
     *t = x.time;
     return x.groups();
@@ -341,7 +338,7 @@ void build_e4m3(const Step& s, int cus, int per_cu, E4m3Lists& out) {
       // 130, whose tiles' lengths differ; nor 64/8, 2048 behind 8000 572 / 606,
       // two tiles a slot).
       if (2 * shortest < longest || x.size() >= 2 * (std::size_t)n) continue;
-      const Shares y(x, n, 1, c);
+      const Shares y(x, n, c);
       if (y.time + c.cut * y.cut_pieces / n < *t) {
         *t = y.time + c.cut * y.cut_pieces / n;
         best = y.groups();
