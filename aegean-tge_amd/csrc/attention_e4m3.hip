@@ -22,6 +22,27 @@
 //   O^T += V^T.P^T  the same instruction: P is already in operand order, and
 //                 V's order in the page gives lane (c, h) the same tokens
 // No value crosses lanes until a tile ends.
+//
+// Roundings: q to f16 once (a score moves by 2^-11 of the sum of its products'
+// magnitudes), weights to f16; sums, bases and accumulators are fp32, out is
+// rounded once.
+//
+// What bounds it, MI355X, 28/4 heads of 128 dims unless said:
+//   decode   the block reads (a probe that only reads blocks of this size 6.6
+//            TB/s). 128 sessions of 8192 tokens 168 us, 6.4 TB/s; 64 ragged
+//            ones of 1k to 32k tokens, four drafted tokens each (613 MB), 118
+//            us, 5.2 TB/s, no matter how the shares are cut, the rest being
+//            starts and merges of 1.4 pieces a workgroup; 32 sessions of 16/8
+//            heads of 256 dims (1234 MB) 223 us, 5.5 TB/s.
+//   prompts  issue: with the matrix cores 40 % and the vector units 50 % of the
+//            time busy, converting the codes and the exponentials stand
+//            between the products. 8192 tokens 460 us, 1046 TFLOP/s; 2048
+//            behind 8000 of 64/8 heads 562 us, 1078; 1333 behind 14003 300 us,
+//            935 (a large f16 product of a library reaches 1105 here).
+//   few rows the chain of loads: item, block numbers, scales, blocks, merge.
+//            One new token at 1056 of 14/2 heads of 64 dims 9.6 us.
+// Rows of a tile, us at RW 1 / 2 / 4: 512 behind 1536 tokens 24 / 31 / 42, 2048
+// tokens 56 / 49 / 50, 8192 tokens 567 / 508 / 470.
 #include <type_traits>
 
 #include "attn_common.h"
@@ -41,7 +62,7 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <int W>
 struct E4m3Cfg {
   static constexpr int BLOCK = e4m3_block_bytes(W);
-  static constexpr int PER_CU = W > 128 ? 1 : W > 64 ? 2 : 3;  // workgroups (= waves per SIMD)
+  static constexpr int PER_CU = W > 128 ? 1 : W > 64 ? 2 : 3;  // workgroups a unit that their LDS leaves room for
   // At 256 dims a tile's codes do not fit beside the accumulators: they are
   // read where they are used, and a wave's own slots refilled by halves (K, V).
   static constexpr bool LAZY = W > 128;

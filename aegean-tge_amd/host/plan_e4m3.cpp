@@ -48,11 +48,14 @@ struct Costs {
 
 // A decode page is bound by HBM (a slot's share of 5.6 TB/s), a prompt page by
 // the matrix cores and the exponentials; waves that share their pages (a larger
-// rw) pay less for the copies. Fitted at 28/4 heads of 128 dims, rw 1 / 2 / 4,
-// us measured (by this model): 2048 tokens 61 / 52 / 51 (59 / 53 / 53), 512
-// behind 1536 25 / 32 / 47 (25 / 31 / 53), 1333 behind 14003 uncut 363 / 388 /
-// 431 (379 / 406 / 412). A cut piece: 4096 tokens at rw 4 uncut 140 us, in halves
-// 162; at rw 2 144 and 168. In 256-dim blocks a compute unit holds one workgroup.
+// rw) pay less for the copies. From launches of 28/4 heads of 128 dims, two
+// workgroups a unit (us at rw 1 / 2 / 4: 2048 tokens 56 / 49 / 50, 512 behind
+// 1536 24 / 31 / 42, 8192 tokens 567 / 508 / 470, 1333 behind 14003 in shares
+// 328 / 318 / 300) a page costs a workgroup 0.15-0.16 / 0.27-0.30 / 0.51-0.58.
+// 64-dim blocks, three workgroups a unit, take two thirds of that (32/8 heads,
+// 4096 tokens 104 / 92 / 90), 256-dim ones, one a unit, as much (16/8 heads, 1000
+// behind 9000 218 / 207 / 199). A cut piece: 4096 tokens of 28/4 heads at rw 4
+// uncut 138, in halves 162; at rw 2 143 and 168.
 Costs costs_of(int rw, bool prompt, int width, int slots) {
   if (!prompt) return Costs{32.0 * width * slots / 5.6e6, 4.5, 2.0, 4.0, 0.25, 0.05, 8, 40, 1};
   const double page = rw == 1 ? 0.155 : rw == 2 ? 0.285 : 0.53;

@@ -499,6 +499,64 @@ def test_captured_calls_replay(gpu):
     tk.hip().ok(h.hipStreamDestroy(st), "destroy")
 
 
+def test_captured_wide_attention_replays(gpu):
+    """256-dim blocks size their LDS at the launch: captured, too."""
+    h = tk.hip().h
+    case = M.Case(16, 8, 256, [(900, 1), (40, 3)], seed=39)
+    case.fill(tk.ROWS_F16)
+    append(case, case.step_rows(tk.ROWS_F16), tk.ROWS_F16)
+    q, out = (M.Rows(np.zeros((4, 16 * 256)), tk.ROWS_F16) for _ in range(2))
+    b, st, graph, run = case.plan(), C.c_void_p(), C.c_void_p(), C.c_void_p()
+    tk.hip().ok(h.hipStreamCreate(C.byref(st)), "stream")
+    tk.hip().sync()
+    tk.hip().ok(h.hipStreamBeginCapture(st, 0), "begin")
+    b.attention_rows(case.pool, 0, tk.attention_rows_args(tk.ROWS_F16, q, out), st)
+    tk.hip().ok(h.hipStreamEndCapture(st, C.byref(graph)), "end")
+    tk.hip().ok(h.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)), "instantiate")
+    for _ in range(3):
+        x = M.as_type(case.rng.standard_normal((4, 16 * 256)), tk.ROWS_F16)
+        tk.hip().upload(q.ptr, M.to_bytes(x, tk.ROWS_F16))
+        tk.hip().sync()
+        tk.hip().ok(h.hipGraphLaunch(run, st), "launch")
+        tk.hip().sync()
+        got = out.read()
+        for rows, cache, ctx in ((slice(0, 1), case.cache[0], 900), (slice(1, 4), case.cache[1], 40)):
+            check(got[rows], *M.attend(cache, ctx, x[rows], 16), tk.ROWS_F16)
+    tk.hip().ok(h.hipGraphExecDestroy(run), "destroy")
+    tk.hip().ok(h.hipGraphDestroy(graph), "destroy")
+    tk.hip().ok(h.hipStreamDestroy(st), "destroy")
+
+
+@pytest.mark.parametrize("qh,kvh,hd", [(28, 4, 128), (16, 8, 256), (14, 2, 64)])
+def test_two_batches_on_two_streams(gpu, qh, kvh, hd):
+    """Steps of two batches overlap: each has its own workspace."""
+    h, t = tk.hip().h, tk.ROWS_BF16
+    sides = []
+    for seed, sessions in ((41, [(5000, 2), (100, 1)]), (43, [(3000, 1), (10, 70)])):
+        case = M.Case(qh, kvh, hd, sessions, seed=seed)
+        case.fill(t)
+        append(case, case.step_rows(t), t)
+        n = sum(m for _, m in sessions)
+        q = M.as_type(case.rng.standard_normal((n, qh * hd)), t)
+        st = C.c_void_p()
+        tk.hip().ok(h.hipStreamCreate(C.byref(st)), "stream")
+        b = tk.Batch().plan(case.pool, [tk.Session(c, m, p) for (c, m), p in zip(case.sessions, case.pages)], qh, st)
+        sides.append((case, q, M.Rows(q, t), [M.Rows(np.zeros_like(q), t) for _ in range(4)], b, st))
+    tk.hip().sync()
+    for i in range(4):
+        for case, _, q, outs, b, st in sides:
+            b.attention_rows(case.pool, 0, tk.attention_rows_args(t, q, outs[i]), st)
+    tk.hip().sync()
+    for case, q, _, outs, _, st in sides:
+        row = 0
+        got = [o.read() for o in outs]
+        assert all(np.array_equal(got[0], g) for g in got[1:])
+        for (c, m), cache in zip(case.sessions, case.cache):
+            check(got[0][row: row + m], *M.attend(cache, c, q[row: row + m], qh), t)
+            row += m
+        tk.hip().ok(h.hipStreamDestroy(st), "destroy")
+
+
 def test_layer_past_4_gib(gpu):
     """A session whose pages sit past the 4 GiB mark of a layer's blocks."""
     pages = 530000  # x 2 heads x 4096 B
