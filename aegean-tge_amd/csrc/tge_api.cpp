@@ -529,8 +529,11 @@ int finish_step_plan(tge_batch* b, hipStream_t st) {
 
 // The e4m3 part of tge_batch_plan: one upload holds
 // [ tables | rows | append tiles | items | merges | counters ].
-int plan_e4m3(tge_batch* b, hipStream_t hs) {
+int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
   const tge::plan::Step& st = b->step;
+  int dev = 0;
+  TGE_HIP(hipGetDevice(&dev));
+  if (dev != pool->device) return fail(TGE_ERR_INVALID, "batch_plan: the pool is on another device");
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
   TGE_HIP(hipStreamIsCapturing(hs, &cs));
   if (cs != hipStreamCaptureStatusNone)
@@ -597,7 +600,7 @@ int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* 
   b->e4.built = false;
 
   hipStream_t hs = static_cast<hipStream_t>(stream);
-  if (pool->desc.format == TGE_KV_E4M3) return plan_e4m3(b, hs);
+  if (pool->desc.format == TGE_KV_E4M3) return plan_e4m3(b, pool, hs);
   // The step's lists are built on the host first and go up in one copy:
   // [ sessions | tables | rows | append tiles | attention lists | step records |
   // first-batch page ids ]. The attention lists are the decode lists when
