@@ -155,11 +155,12 @@ struct AttnPlan {
   size_t off_app = 0;  // app_first, then app_recs (decode plans that store the new rows)
   tge::plan::Scratch part_o;   // [parts][rows_cap][block width] fp32
   tge::plan::Scratch part_ml;  // [parts][rows_cap][2] fp32
-  ~AttnPlan() {
+  void release() {
     image.release(g_mem);
     part_o.release(g_mem);
     part_ml.release(g_mem);
   }
+  ~AttnPlan() { release(); }
 };
 
 // A small decode step in one launch (paged_step_kernel): its records, the
@@ -170,11 +171,12 @@ struct StepPlan {
   bool built = false;
   char* dev = nullptr;  // records | first-batch page ids, in the batch image
   tge::plan::Scratch part_o, part_ml, counters;
-  ~StepPlan() {
+  void release() {
     part_o.release(g_mem);
     part_ml.release(g_mem);
     counters.release(g_mem);
   }
+  ~StepPlan() { release(); }
 };
 
 // A step on an e4m3 pool: everything that its append and attention launches
@@ -184,10 +186,11 @@ struct E4m3Plan {
   bool built = false;
   size_t off_tiles = 0, off_items = 0, off_merges = 0, off_counters = 0;  // in the batch image
   tge::plan::Scratch part_o, part_ml;
-  ~E4m3Plan() {
+  void release() {
     part_o.release(g_mem);
     part_ml.release(g_mem);
   }
+  ~E4m3Plan() { release(); }
 };
 
 }  // namespace
@@ -199,6 +202,7 @@ struct tge_batch {
   // The pool's storage the plan was built for (the one-launch step's page
   // batches depend on it).
   int format = 0, scale_format = 0;
+  int device = -1;  // of the plan and its buffers
   AttnPlan decode, prefill;
   E4m3Plan e4;
   // Mixed steps (tge_batch_attention): the decode kernel over the sessions
@@ -224,13 +228,21 @@ struct tge_batch {
   std::vector<char> prof_merged;  // whether the call launched the split merge kernel
   size_t prof_used = 0;
 
-  ~tge_batch() {
+  // Everything that lives on `device` (a plan on another one starts anew).
+  void release() {
     image.release(g_mem);
     mix_counters.release(g_mem);
+    for (AttnPlan* p : {&decode, &prefill, &mix_decode, &mix_prefill}) p->release();
+    small.release();
+    e4.release();
     for (auto& t : prof)
       for (hipEvent_t e : t)
         if (e) (void)hipEventDestroy(e);
+    prof.clear();
+    prof_merged.clear();
+    prof_used = 0;
   }
+  ~tge_batch() { release(); }
 };
 
 namespace {
@@ -527,6 +539,22 @@ int finish_step_plan(tge_batch* b, hipStream_t st) {
   return TGE_OK;
 }
 
+// Before a plan on the current device: buffers that an earlier plan left on
+// another one go, once that device has finished with them.
+int move_to_current_device(tge_batch* b) {
+  int dev = 0;
+  TGE_HIP(hipGetDevice(&dev));
+  if (b->device != dev && b->device >= 0) {
+    TGE_HIP(hipSetDevice(b->device));
+    const hipError_t e = hipDeviceSynchronize();
+    if (e == hipSuccess) b->release();
+    TGE_HIP(hipSetDevice(dev));
+    TGE_HIP(e);
+  }
+  b->device = dev;
+  return TGE_OK;
+}
+
 // The e4m3 part of tge_batch_plan: one upload holds
 // [ tables | rows | append tiles | items | merges | counters ].
 int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
@@ -540,6 +568,8 @@ int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
     return fail(TGE_ERR_INVALID,
                 "batch_plan: the stream is capturing (the plan is uploaded from host memory, which a "
                 "graph would replay stale; plan first, then capture the calls)");
+  int s = move_to_current_device(b);
+  if (s != TGE_OK) return s;
   E4m3Plan& e = b->e4;
   try {
     tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
@@ -555,7 +585,7 @@ int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
   e.off_merges = align_up(e.off_items + L.items.size() * sizeof(tge::E4m3Item));
   e.off_counters = align_up(e.off_merges + L.merges.size() * sizeof(tge::E4m3Merge));
   const size_t total = e.off_counters + L.merges.size() * sizeof(int);
-  int s = b->image.upload(g_mem, total, hs, [&](char* h) {
+  s = b->image.upload(g_mem, total, hs, [&](char* h) {
     auto put = [&](size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(h + at, v.data(), v.size() * sizeof(v[0]));
     };
@@ -601,6 +631,8 @@ int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* 
 
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (pool->desc.format == TGE_KV_E4M3) return plan_e4m3(b, pool, hs);
+  s = move_to_current_device(b);
+  if (s != TGE_OK) return s;
   // The step's lists are built on the host first and go up in one copy:
   // [ sessions | tables | rows | append tiles | attention lists | step records |
   // first-batch page ids ]. The attention lists are the decode lists when
@@ -857,6 +889,7 @@ int check_e4m3(const tge_batch* b, const tge_kv_pool* p, const char* who) {
   int dev = 0;
   TGE_HIP(hipGetDevice(&dev));
   if (dev != p->device) return fail(TGE_ERR_INVALID, std::string(who) + ": the pool is on another device");
+  if (dev != b->device) return fail(TGE_ERR_INVALID, std::string(who) + ": the batch was planned on another device");
   return TGE_OK;
 }
 

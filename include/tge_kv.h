@@ -359,7 +359,9 @@ int tge_batch_attention(const tge_batch* batch, const tge_kv_pool* pool,
  * tge_decode_attention_static, tge_attention_group and a static sparse subset
  * are refused on such a pool (TGE_ERR_INVALID), and so are these two calls on
  * any other pool, on a pool of another device than the current one (its plans
- * too), and tge_batch_plan on a stream that is capturing. The calls themselves launch
+ * too) or with a plan made on another device (of a pool of the same shape there),
+ * and tge_batch_plan on a stream that is capturing. A batch planned anew on
+ * another device takes its buffers there. The calls themselves launch
  * one kernel each and may be captured; a captured call stays valid until its
  * batch is planned again or destroyed. The plan holds the workspace: calls on
  * one batch must not overlap on the device (two streams, or two graphs).
