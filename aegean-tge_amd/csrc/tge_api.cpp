@@ -12,7 +12,6 @@
 #include <functional>
 #include <mutex>
 #include <stdexcept>
-#include <new>
 #include <string>
 #include <array>
 #include <vector>
@@ -571,11 +570,7 @@ int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
   int s = move_to_current_device(b);
   if (s != TGE_OK) return s;
   E4m3Plan& e = b->e4;
-  try {
-    tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
-  } catch (const std::bad_alloc&) {
-    return fail(TGE_ERR_CAPACITY, "batch_plan: out of host memory");
-  }
+  tge::plan::build_e4m3(st, device_cus(), tge::e4m3_groups_per_cu(st.block_dims), e.lists);
   const auto& L = e.lists;
   if ((size_t)L.parts * L.part_rows * st.block_dims * sizeof(float) > 0x7fffffffu)
     return fail(TGE_ERR_CAPACITY, "batch_plan: the step's partial states exceed 2 GiB");
@@ -608,11 +603,7 @@ int plan_e4m3(tge_batch* b, const tge_kv_pool* pool, hipStream_t hs) {
   return TGE_OK;
 }
 
-}  // namespace
-
-int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* d,
-                   void* stream) {
-  if (!b || !pool || !d) return fail(TGE_ERR_INVALID, "batch_plan: null argument");
+int plan_batch(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* d, void* stream) {
   const int hd = pool->desc.head_dim;
   const char* msg = nullptr;
   b->planned = false;
@@ -697,6 +688,18 @@ int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* 
   }
   b->planned = true;
   return TGE_OK;
+}
+
+}  // namespace
+
+int tge_batch_plan(tge_batch* b, const tge_kv_pool* pool, const tge_batch_desc* d,
+                   void* stream) {
+  if (!b || !pool || !d) return fail(TGE_ERR_INVALID, "batch_plan: null argument");
+  try {
+    return plan_batch(b, pool, d, stream);
+  } catch (const std::exception&) {  // (host memory, or a list longer than any)
+    return fail(TGE_ERR_CAPACITY, "out of memory");  // (short enough to need none)
+  }
 }
 
 int tge_batch_info(const tge_batch* b, int* rows, int* work_items, int* max_splits) {

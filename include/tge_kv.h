@@ -195,7 +195,7 @@ void tge_batch_destroy(tge_batch* batch);
 
 /* Validates the description against `pool`, builds the work lists and
  * uploads tables and plan (one host-to-device copy on `stream`). A failure
- * leaves the batch unplanned; TGE_ERR_CAPACITY when device or pinned host
+ * leaves the batch unplanned; TGE_ERR_CAPACITY when device or host
  * memory runs out (a later, smaller plan allocates again). */
 int tge_batch_plan(tge_batch* batch, const tge_kv_pool* pool,
                    const tge_batch_desc* desc, void* stream);

@@ -6,9 +6,13 @@
 //   devices  calls on an e4m3 pool with a plan made on another device are
 //            refused, for a pool of the same shape, too; a batch planned anew on
 //            another device has its buffers there
+//   memory   host memory that runs out anywhere in tge_batch_plan comes back as
+//            TGE_ERR_CAPACITY, no exception leaves the call, the batch has no
+//            plan, and the same plan succeeds afterwards
 // Prints "api_check ok" or the first failure (exit 1).
 #include <cstdio>
 #include <cstdlib>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -25,6 +29,27 @@
       std::exit(1);                                            \
     }                                                          \
   } while (0)
+
+// ---- host memory that runs out at the n-th allocation ------------------------------
+namespace {
+long g_until_failure = -1;  // allocations that still succeed (-1: all)
+void* allocate(std::size_t n) {
+  if (g_until_failure == 0) throw std::bad_alloc();
+  if (g_until_failure > 0) --g_until_failure;
+  void* p = std::malloc(n ? n : 1);
+  if (!p) throw std::bad_alloc();
+  return p;
+}
+}  // namespace
+void* operator new(std::size_t n) { return allocate(n); }
+void* operator new[](std::size_t n) { return allocate(n); }
+void* operator new(std::size_t n, const std::nothrow_t&) noexcept {
+  return g_until_failure == 0 ? nullptr : std::malloc(n ? n : 1);
+}
+void operator delete(void* p) noexcept { std::free(p); }
+void operator delete[](void* p) noexcept { std::free(p); }
+void operator delete(void* p, std::size_t) noexcept { std::free(p); }
+void operator delete[](void* p, std::size_t) noexcept { std::free(p); }
 
 // ---- the launchers --------------------------------------------------------------
 namespace {
@@ -197,12 +222,52 @@ void check_devices() {
   REQUIRE(fake_hip::state().live.empty(), "%zu allocations left", fake_hip::state().live.size());
 }
 
+void check_memory() {
+  // (a decoding step cut into pieces, a prompt, both)
+  for (const Sessions& s : {Sessions({{9000, 2}, {40, 1}}), Sessions({{100, 300}}), Sessions({{3000, 1}, {0, 200}})})
+    for (int format : {TGE_KV_E4M3, TGE_KV_F16, TGE_KV_I8}) {
+      const tge_batch_desc d = s.desc(8);
+      alignas(16) static float x[4096];
+      tge_kv_pool* pool = pool_on(0, format);
+      int failures = 0;
+      for (long n = 0;; ++n) {
+        tge_batch* b = nullptr;
+        REQUIRE(tge_batch_create(&b) == TGE_OK, "create");
+        g_until_failure = n;
+        int status = TGE_OK;
+        bool left = false;
+        try {
+          status = tge_batch_plan(b, pool, &d, nullptr);
+        } catch (...) {
+          left = true;
+        }
+        const bool all = g_until_failure > 0;  // (the plan needed fewer)
+        g_until_failure = -1;
+        REQUIRE(!left, "format %d: an exception left the plan at allocation %ld", format, n);
+        if (status != TGE_OK) {
+          REQUIRE(status == TGE_ERR_CAPACITY, "format %d, allocation %ld: status %d", format, n, status);
+          REQUIRE(std::string(tge_last_error()).find("memory") != std::string::npos, "%s", tge_last_error());
+          REQUIRE(tge_kv_append(b, pool, 0, x, x, nullptr) == TGE_ERR_INVALID, "a call after a failed plan");
+          REQUIRE(tge_batch_plan(b, pool, &d, nullptr) == TGE_OK, "%s", tge_last_error());
+          ++failures;
+        }
+        REQUIRE(tge_kv_append(b, pool, 0, x, x, nullptr) == TGE_OK, "%s", tge_last_error());
+        tge_batch_destroy(b);
+        if (all) break;
+      }
+      REQUIRE(failures > 5, "%d failures", failures);
+      tge_kv_pool_destroy(pool);
+    }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const std::string which = argc > 1 ? argv[1] : "";
   if (which == "devices")
     check_devices();
+  else if (which == "memory")
+    check_memory();
   else
     REQUIRE(false, "unknown check");
   std::printf("api_check ok\n");

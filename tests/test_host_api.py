@@ -34,3 +34,8 @@ def test_calls_stay_on_their_device(api_check):
     """A call whose plan or pool is on another device is refused, and a batch
     planned anew on another device has its buffers there."""
     api_check("devices")
+
+
+def test_plan_without_host_memory(api_check):
+    """tge_batch_plan returns TGE_ERR_CAPACITY wherever host memory runs out."""
+    api_check("memory")
