@@ -21,7 +21,11 @@
 //                 is taken from the rounded weights, in fp32
 //   O^T += V^T.P^T  the same instruction: P is already in operand order, and
 //                 V's order in the page gives lane (c, h) the same tokens
-// No value crosses lanes until a tile ends.
+// No accumulator and no weight crosses lanes until a tile ends.
+//
+// Every row sees its own position, so its weights sum to more than 0 unless all
+// its scores are -infinity (an infinite q against K of the other sign): 0 / 0
+// makes that row NaN, as the formula does.
 //
 // Roundings: q to f16 once (a score moves by 2^-11 of the sum of its products'
 // magnitudes), weights to f16; sums, bases and accumulators are fp32, out is
@@ -411,8 +415,7 @@ __device__ __forceinline__ void merge_parts(const E4m3Attn& p, E4m3Shared<W>& sh
     for (int j = 0; j < J; ++j) {
       const int idx = i0 + 256 * j, r = idx / (W / 4), d4 = idx % (W / 4);
       if (idx < chunks && 4 * d4 < p.dims)
-        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
-                   sum[j] > 0.0f || sum[j] != sum[j] ? div4(acc[j], sum[j]) : float4_t{0, 0, 0, 0});
+        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type, div4(acc[j], sum[j]));
     }
   }
   if (t == 0) __hip_atomic_store(p.counters + it.merge, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -624,10 +627,7 @@ __device__ __forceinline__ void finish_item(const E4m3Attn& p, E4m3Shared<W>& sh
     float4_t acc = *reinterpret_cast<const float4_t*>(from);
     for (int k = 1; k < copies; ++k) acc += *reinterpret_cast<const float4_t*>(from + k * rw * 32 * W * 4);
     if (it.part < 0) {
-      const float sum = sh.sum[r];
-      if (4 * d4 < p.dims)
-        store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type,
-                   sum > 0.0f || sum != sum ? div4(acc, sum) : float4_t{0, 0, 0, 0});
+      if (4 * d4 < p.dims) store_out4(p.out, sh.out_at[r] + 4 * d4, p.row_type, div4(acc, sh.sum[r]));
     } else {
       coh_store4(rs_o, (uint32_t)((((size_t)it.part * p.part_rows + r) * W + 4 * d4) * 4), acc);
       if (d4 == 0) coh_store2(rs_ml, (uint32_t)(((size_t)it.part * p.part_rows + r) * 8), sh.base[r], sh.sum[r]);

@@ -416,8 +416,8 @@ typedef struct {
  * q is scaled and rounded to f16 once (rows of f16 enter as they are, the
  * scores are scaled; a scaled value past f16's largest, 65504, counts as
  * infinite), softmax weights are f16, sums and accumulators fp32, out is
- * rounded once. A row of NaN gives NaN and touches no other row. The same
- * inputs give the same bits on every run. */
+ * rounded once. A row of q with a NaN or an infinity gives NaN and touches no
+ * other row. The same inputs give the same bits on every run. */
 int tge_attention_rows(const tge_batch* batch, const tge_kv_pool* pool, int layer,
                        const tge_attention_rows_args* args, void* stream);
 

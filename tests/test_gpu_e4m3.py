@@ -310,6 +310,48 @@ def test_nan_rows_stay_alone(gpu):
     assert not bad.any()
 
 
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_infinite_queries_give_nan(gpu, hd, row_type):
+    """A row whose q holds an infinity (or, scaled, a value past f16's largest)
+    is NaN whether its scores are all +inf or all -inf; the rows around it are
+    what they are without it. One visible position, a part of a page, a context
+    in pieces, a prompt."""
+    qh, kvh, bad = 4, 2, 3
+    case = M.Case(qh, kvh, hd, [(0, 1), (40, 2), (9000, 2), (5, 70)], seed=hd)
+    plain = case.rows
+
+    def rows(n, t):  # (dim `bad` of every K row is positive)
+        k, v = plain(n, t)
+        k[:, bad::hd] = M.as_type(np.abs(k[:, bad::hd]) + 1.0, t)
+        return k, v
+
+    case.rows = rows
+    case.fill(row_type)
+    b = append(case, case.step_rows(row_type), row_type)
+    assert b.info()[2] > 1
+    n = sum(m for _, m in case.sessions)
+    q = M.as_type(case.rng.standard_normal((n, qh * hd)), row_type)
+    past = np.inf if row_type == tk.ROWS_F16 else 1e7
+    want_nan = np.zeros((n, qh), bool)
+    sent = q.copy()
+    for i in range(n):
+        for h in range(qh):
+            if (i + h) % 3 == 0:
+                want_nan[i, h] = True
+                sent[i, h * hd + bad] = [np.inf, -np.inf, past, -past][(i // 3 + h) % 4]
+    dq, out = M.Rows(sent, row_type), M.Rows(np.zeros_like(q), row_type)
+    b.attention_rows(case.pool, 0, tk.attention_rows_args(row_type, dq, out))
+    tk.hip().sync()
+    got, row = out.read().reshape(n, qh, hd), 0
+    assert np.isnan(got[want_nan]).all(), np.argwhere(want_nan & ~np.isnan(got).all(-1))
+    for (c, m), cache in zip(case.sessions, case.cache):
+        want, bound = (x.reshape(m, qh, hd) for x in M.attend(cache, c, q[row: row + m], qh))
+        live = ~want_nan[row: row + m]
+        check(got[row: row + m][live], want[live], bound[live], row_type)
+        row += m
+
+
 def test_stale_pages_do_not_reach_a_row(gpu):
     """Every byte of the pool is a NaN code before the step is stored."""
     case = M.Case(8, 2, 128, [(0, 5), (0, 33)], seed=19)
