@@ -404,6 +404,28 @@ def test_copy_page(gpu):
     assert np.array_equal(scales[free], scales[case.pages[0][1]])
 
 
+def test_copy_page_in_every_layer(gpu):
+    """Codes and scales of the page in each layer, and nothing else."""
+    case = M.Case(6, 3, 64, [(20, 4)], seed=45, layers=3)
+    for layer in range(3):
+        case.cache = [M.Cache(3, 64)]
+        case.fill(layer=layer)
+        rows = [(k * np.float32(4.0 ** layer), v) for k, v in case.step_rows(tk.ROWS_F32)]
+        append(case, rows, tk.ROWS_F32, layer=layer)
+    free = case.table.allocate()
+    before = [M.raw_layer(case.pool, layer) for layer in range(3)]
+    source = case.pages[0][1]
+    case.pool.copy_page(source, free)
+    for layer, (codes, scales) in enumerate(before):
+        codes[free], scales[free] = codes[source], scales[source]
+        got = M.raw_layer(case.pool, layer)
+        assert np.array_equal(got[0], codes) and np.array_equal(got[1], scales), layer
+        assert codes[free].any() and scales[free].any()
+    # (the layers' pages differ, so that one layer's copy cannot pass for another's)
+    assert not np.array_equal(before[0][1][source], before[1][1][source])
+    assert not np.array_equal(before[1][1][source], before[2][1][source])
+
+
 def test_driver_serves_16_bit_rows(gpu):
     """The Qwen2-shaped driver over steps of a session: prompt, decode, drafts
     that are rejected, decode again, every step against the model."""
