@@ -27,24 +27,33 @@
 // its scores are -infinity (an infinite q against K of the other sign): 0 / 0
 // makes that row NaN, as the formula does.
 //
-// Roundings: q to f16 once (a score moves by 2^-11 of the sum of its products'
-// magnitudes), weights to f16; sums, bases and accumulators are fp32, out is
-// rounded once.
+// Roundings: rows of fp32 and bf16 are scaled and rounded to f16 once (a score
+// moves by 2^-11 of the sum of its products' magnitudes, and by 2^-25 of the sum
+// of |k| where scaled values lie below f16's normal range), rows of f16 enter as
+// they are and their scores are scaled; weights are rounded to f16; sums, bases
+// and accumulators are fp32, out is rounded once.
 //
 // What bounds it, MI355X, 28/4 heads of 128 dims unless said:
 //   decode   the block reads (a probe that only reads blocks of this size 6.6
-//            TB/s). 128 sessions of 8192 tokens 168 us, 6.4 TB/s; 64 ragged
-//            ones of 1k to 32k tokens, four drafted tokens each (613 MB), 118
-//            us, 5.2 TB/s, no matter how the shares are cut, the rest being
-//            starts and merges of 1.4 pieces a workgroup; 32 sessions of 16/8
-//            heads of 256 dims (1234 MB) 223 us, 5.5 TB/s.
+//            TB/s). 128 sessions of 8192 tokens 164-168 us, 6.4-6.6 TB/s; 64
+//            ragged ones of 1k to 32k tokens, four drafted tokens each (613 MB),
+//            118-121 us, 5.1-5.2 TB/s, no matter how the shares are cut, the
+//            rest being starts and merges of 1.4 pieces a workgroup; 32 sessions
+//            of 16/8 heads of 256 dims (1234 MB) 219-225 us, 5.5-5.6 TB/s. With
+//            33 to 64 rows a KV head the conversions and products count too: 64
+//            such sessions of 64/8 heads, eight drafted tokens each (1236 MB),
+//            253 us, 4.9 TB/s.
 //   prompts  issue: with the matrix cores 40 % and the vector units 50 % of the
 //            time busy, converting the codes and the exponentials stand
-//            between the products. 8192 tokens 460 us, 1046 TFLOP/s; 2048
-//            behind 8000 of 64/8 heads 562 us, 1078; 1333 behind 14003 300 us,
-//            935 (a large f16 product of a library reaches 1105 here).
-//   few rows the chain of loads: item, block numbers, scales, blocks, merge.
-//            One new token at 1056 of 14/2 heads of 64 dims 9.6 us.
+//            between the products. 8192 tokens 460-487 us, 990-1046 TFLOP/s; 2048
+//            behind 8000 of 64/8 heads 562-596 us, 1015-1078; 1333 behind 14003
+//            300-316 us, 887-935 (a large f16 product of a library reaches 1105
+//            here). Shorter ones lack work to even out causal tiles of unlike
+//            lengths: 2048 tokens 49 us, 608 TFLOP/s; so do those of 256 dims,
+//            one workgroup a unit: 2048 of 16/8 heads 70 us, 489.
+//   few rows the chain of loads: item, block numbers, scales and blocks, then
+//            the waves' turns, and a merge where the context is cut. One new
+//            token at 1056 of 14/2 heads of 64 dims (uncut) 9.0-9.6 us.
 // Rows of a tile, us at RW 1 / 2 / 4: 512 behind 1536 tokens 24 / 31 / 42, 2048
 // tokens 56 / 49 / 50, 8192 tokens 567 / 508 / 470.
 #include <type_traits>

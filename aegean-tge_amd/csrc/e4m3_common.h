@@ -85,12 +85,13 @@ struct E4m3Item {
 };
 static_assert(sizeof(E4m3Item) == 16 * sizeof(int), "E4m3Item is read as 16 ints");
 
+// A cut tile: the last of its pieces to arrive merges them all.
 struct E4m3Merge {
   int first_part;
   int n_parts;
   int rows;
-  int row0;
-  int kv_head;
+  int row0;     // which tile it is: for checks of a plan (the kernel knows from
+  int kv_head;  // the arriving piece)
   int q_row;
   int pad[2];
 };

@@ -393,7 +393,9 @@ typedef struct {
 /* Store the step's new rows. Per block that receives some: e is the smallest
  * exponent with max|x| <= 448 * 2^e over the block's new rows, at least -15, at
  * most 7, and, where the block holds rows of positions before the step, not
- * below their exponent. A value is stored as the code nearest x * 2^-e (ties to
+ * below the exponent stored with it. (That one stays after the rows that set it
+ * are dropped, rejected drafts for instance, and so do older codes re-encoded
+ * for them, until the block's first slot is written again.) A value is stored as the code nearest x * 2^-e (ties to
  * even), out of range as the largest code, a NaN as zero (stored values are
  * finite, so no masked position can reach a row); older codes are re-encoded
  * where e grew. The page's slots behind the last new row are cleared: rows
